@@ -21,7 +21,10 @@ HEADERS = ["common.h", "kernels.h", "gemm_tile.h", "attention_w4_body.inc", "att
 # float(bf16(a*b)) + float(c) to bf16 fmul/fadd and the default -ffp-contract=fast then fuses them
 # into one fma, silently deleting a bf16 rounding the reference performs (measured: 29 % of
 # ln_modulate outputs off by one ulp).  Fusion is written explicitly (fmaf) where it is wanted.
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++20", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function"]
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 out of ordinary float code (some of their forms have given wrong results now and then, and
+# beside MFMAs they are slower than two plain instructions); the host pass warns that it does not know the feature, which is harmless.
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++20", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # per-source extras.  attention.hip: no SLP vectorisation -- it turns adjacent fp32 adds / muls / fmas of the softmax into v_pk_*_f32, which
 # on gfx950 costs more than the two plain VALU it replaces when issued beside MFMAs
 # gemm.hip (round 6): the deferred epilogue's slices run beside the other wave group's MFMAs and are written in scalar fp32 for the same reason
@@ -80,8 +83,9 @@ def build(force: bool = False, verbose: bool = True) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"hipcc failed for {src}:\n{r.stdout}\n{r.stderr}")
-        if verbose and r.stderr.strip():
-            print(r.stderr, file=sys.stderr)
+        notes = "\n".join(ln for ln in r.stderr.splitlines() if "packed-fp32-ops" not in ln).strip()
+        if verbose and notes:
+            print(notes, file=sys.stderr)
         return obj
 
     if jobs:
