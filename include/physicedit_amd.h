@@ -292,6 +292,93 @@ int pe_decode_layer(const pe_decode_layer_weights* w, const void* x, void* x_out
                     void* v_cache, const int* step, int base_len, int cache_len, float scale, void* scratch, size_t scratch_bytes, void* stream);
 int pe_decode_embed(const void* table, const int* token, void* x, int dim, int vocab, void* stream);
 int pe_decode_argmax(const void* logits, int vocab, int* token, int* out_ids, int* step, int max_steps, void* stream);
+/* ---------------------------------------------------------------------------------------------
+ * The low-bit decode step: linears with 4-bit weights, an e4m3 key/value cache, next-token scores.  Not part of the reference (its text
+ * encoder decodes in bf16): opt-in operators beside pe_gemv_* / pe_decode_*, used by GraphDecoder(weights="w4", kv_cache="e4m3",
+ * penalties / masks).  Sums, softmax statistics and scales are fp32; outputs are rounded once.  None of them keeps state between calls
+ * or uses an atomic whose order changes a result.
+ * ------------------------------------------------------------------------------------------- */
+
+/* A weight [N,K] of 4-bit codes, value = scale * (code - zero) with one scale (bf16) and zero point per output and `group` inputs
+ * (32, 64 or 128; K a multiple of it), laid out once (ops.pack_w4 / ops.quantize_w4 write it):
+ *   codes  [ceil(N/16)][ceil(K/128)][64][4] words, 16-byte aligned: word s of lane l holds output l % 16 of the tile, inputs 32 s + 8 (l / 16) + e of the
+ *          chunk, element e in nibble e / 2 + 4 (e % 2);
+ *   scale  [ceil(N/16)][128 / group * ceil(K/128)][16] bf16, 0 for outputs >= N and inputs >= K;  zero: the same shape in bytes, NULL = 8 everywhere. */
+typedef struct pe_w4_weight {
+    const void *codes, *scale, *zero;
+    int N, K, group;
+} pe_w4_weight;
+/* out[M, N] = r * (x @ W^T) + bias + res for 1 ... 64 rows x [M,K] bf16 (finite values; row stride ldx, a multiple of 8; 16-byte aligned).  norm_eps >= 0:
+ * r[m] = rsqrt(mean(x[m]^2) + norm_eps), an RMSNorm whose weight the caller folded into W; norm_eps < 0: r = 1.  bias [N], res [M, N] (row
+ * stride ldr; may be out itself) nullable.  swiglu != 0: W holds the F = N / 2 gate rows, then the F up rows (F % 16 == 0), and
+ * out[M, F] = silu(gate) * up (no res). */
+int pe_gemv_w4(const void* x, long long ldx, int M, const pe_w4_weight* w, const void* bias, const void* res, long long ldr, void* out,
+               long long ldo, int swiglu, float norm_eps, void* stream);
+
+/* The cache of one layer: rows of (sequence, token, kv head), value = e4m3fn code * scale.  k [batch][n_kv][capacity][head_dim] bytes,
+ * v [batch][n_kv][capacity/64][head_dim][64] bytes (blocks of 64 tokens, transposed), scales [batch][n_kv][capacity] fp32, all 16-byte aligned and
+ * zero when first used; capacity % 64 == 0, head_dim 64 or 128. */
+typedef struct pe_kv_cache {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int batch, n_kv, capacity, head_dim;
+} pe_kv_cache;
+/* Writes T tokens of every sequence at cache rows start[b] + t (start: device int32 [batch]); rows at or past the capacity, and all of a sequence
+ * with start[b] < 0, are not written.  scale = max(max|row| * (1/448), 2^-126), code = e4m3(value / scale); a row with a value that is not
+ * finite gets the scale NaN and codes of 0 (it makes every output that sees it NaN, and none that does not).
+ * k, v (and q) bf16 [batch][T][heads][head_dim] with strides {batch, token, head} in elements (multiples of 8), channels contiguous, 16-byte aligned.
+ * cos / sin [table_rows][head_dim] (bf16, or fp32 with table_f32 != 0), NULL = no rotation: k and q are rotated first, x * cos + rotate_half(x) * sin in
+ * fp32, with table row positions[b][t] (device int32, NULL = start[b] + t); a row outside the tables makes the token's k and q NaN.
+ * q_out [batch][T][n_q][head_dim] bf16: the rotated queries; zeros for tokens that are not written.  n_q = 0: no queries. */
+typedef struct pe_kv_append_args {
+    const void *q, *k, *v;
+    long long q_strides[3], k_strides[3], v_strides[3];
+    void* q_out;
+    const void *cos, *sin;
+    int table_rows, table_f32;
+    const int *positions, *start;
+    int T, n_q;
+} pe_kv_append_args;
+int pe_kv_append_e4m3(const pe_kv_cache* cache, const pe_kv_append_args* a, void* stream);
+/* Attention of the T (1 ... 64) newest tokens, already appended at rows start[b] + t: query (b, t, h) sees the cache rows [0, start[b]) and the row
+ * start[b] + j of every new token j with bit j of tree[b][t] set (device uint64 [batch][T]: the token's ancestors and, usually, itself); tree NULL =
+ * causal.  Grouped heads: query head h reads kv head h / (n_q / n_kv).  softmax in fp32; a query that sees nothing, or start[b] < 0: zeros.
+ * q bf16 with strides {batch, token, head} (multiples of 8), out [batch][T][n_q][head_dim] bf16.  workspace: pe_kv_attention_workspace_bytes, 16-byte
+ * aligned, private to the stream (a captured graph keeps its own). */
+size_t pe_kv_attention_workspace_bytes(int batch, int n_kv, int T, int n_q, int head_dim, int capacity);
+int pe_kv_attention_e4m3(const pe_kv_cache* cache, const void* q, const long long* q_strides, const int* start, const void* tree, int T, int n_q,
+                         float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Scores [rows][vocab] (bf16, or fp32 with f32 != 0; row stride ld) with, in this order and in fp32:
+ *   counts[row][v] != 0 (int16: bit 15 = the prompt holds v, bits 0 ... 14 = how often it was generated): l > 0 ? l / repetition : l * repetition
+ *   l -= frequency * generated;  l -= presence * (generated > 0);  l += bias[v];  mask bit v (word v / 32, bit v % 32) clear: -inf, whatever l was
+ * penalties [rows][3] fp32: repetition, presence, frequency.  Every table is nullable; penalties need counts.  Row strides of penalties, bias
+ * and allowed may be 0: one row for all. */
+typedef struct pe_logits_args {
+    const void* logits;
+    long long ld;
+    int f32, rows, vocab;
+    void* counts;
+    long long ld_counts;
+    const float* penalties;
+    long long ld_penalties;
+    const float* bias;
+    long long ld_bias;
+    const void* allowed;
+    long long ld_allowed;
+} pe_logits_args;
+/* out [rows][vocab] fp32 */
+int pe_process_logits(const pe_logits_args* a, float* out, void* stream);
+/* token[row] = first maximum of the processed scores (NaN is never chosen), -1 where all are -inf.  update_counts != 0: the token's count goes up by one
+ * (it stays at 32767).  step (device, rows == 1 only, nullable): out_ids[*step] = token while *step < max_steps, then *step += 1 -- pe_decode_argmax's
+ * convention.  workspace: pe_select_token_workspace_bytes bytes, private to the stream. */
+size_t pe_select_token_workspace_bytes(int rows, int vocab);
+int pe_select_token(const pe_logits_args* a, int* token, int update_counts, int* out_ids, int* step, int max_steps, void* workspace,
+                    size_t workspace_bytes, void* stream);
+/* counts[row][tokens[row][i]]: prompt != 0 sets bit 15, else the count goes up by one per occurrence (up to 32767).  Ids outside the vocabulary
+ * (padding: -1) are skipped. */
+int pe_token_counts_add(void* counts, long long ld_counts, int rows, int vocab, const int* tokens, int n, int prompt, void* stream);
+
 /* BlockWiseControlBlock input (models/qwen_image_controlnet.py:16-18): out = bf16(RMSNorm(x; wx) + RMSNorm(y; wy)), rows of
  * dim = 3072, each RMSNorm with the roundings of models/utils.py:250-257. */
 int pe_dual_rmsnorm_add(const void* x, const void* wx, const void* y, const void* wy, void* out, int rows, int dim, float eps,

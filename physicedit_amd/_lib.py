@@ -52,6 +52,31 @@ class DecodeLayerWeights(C.Structure):
                                                            ("n_q_heads", c_int), ("n_kv_heads", c_int), ("ff", c_int)]
 
 
+class W4Weight(C.Structure):
+    """pe_w4_weight"""
+    _fields_ = [("codes", c_void_p), ("scale", c_void_p), ("zero", c_void_p), ("N", c_int), ("K", c_int), ("group", c_int)]
+
+
+class KvCache(C.Structure):
+    """pe_kv_cache"""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("batch", c_int), ("n_kv", c_int),
+                ("capacity", c_int), ("head_dim", c_int)]
+
+
+class KvAppendArgs(C.Structure):
+    """pe_kv_append_args"""
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_strides", C.c_longlong * 3), ("k_strides", C.c_longlong * 3),
+                ("v_strides", C.c_longlong * 3), ("q_out", c_void_p), ("cos", c_void_p), ("sin", c_void_p), ("table_rows", c_int),
+                ("table_f32", c_int), ("positions", c_void_p), ("start", c_void_p), ("T", c_int), ("n_q", c_int)]
+
+
+class LogitsArgs(C.Structure):
+    """pe_logits_args"""
+    _fields_ = [("logits", c_void_p), ("ld", C.c_longlong), ("f32", c_int), ("rows", c_int), ("vocab", c_int), ("counts", c_void_p),
+                ("ld_counts", C.c_longlong), ("penalties", c_void_p), ("ld_penalties", C.c_longlong), ("bias", c_void_p),
+                ("ld_bias", C.c_longlong), ("allowed", c_void_p), ("ld_allowed", C.c_longlong)]
+
+
 class VaeConv(C.Structure):
     _fields_ = [("w", c_void_p), ("b", c_void_p), ("cin_p", c_int), ("cout_p", c_int), ("ksize", c_int)]
 
@@ -157,6 +182,16 @@ SIGNATURES = {
                                 c_int, C.c_float, c_void_p, c_size_t, c_void_p]),
     "pe_decode_embed": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "pe_decode_argmax": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "pe_gemv_w4": (c_int, [c_void_p, C.c_longlong, c_int, C.POINTER(W4Weight), c_void_p, c_void_p, C.c_longlong, c_void_p, C.c_longlong,
+                           c_int, c_float, c_void_p]),
+    "pe_kv_append_e4m3": (c_int, [C.POINTER(KvCache), C.POINTER(KvAppendArgs), c_void_p]),
+    "pe_kv_attention_workspace_bytes": (c_size_t, [c_int] * 6),
+    "pe_kv_attention_e4m3": (c_int, [C.POINTER(KvCache), c_void_p, C.POINTER(C.c_longlong), c_void_p, c_void_p, c_int, c_int, c_float,
+                                     c_void_p, c_void_p, c_size_t, c_void_p]),
+    "pe_process_logits": (c_int, [C.POINTER(LogitsArgs), c_void_p, c_void_p]),
+    "pe_select_token_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "pe_select_token": (c_int, [C.POINTER(LogitsArgs), c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "pe_token_counts_add": (c_int, [c_void_p, C.c_longlong, c_int, c_int, c_void_p, c_int, c_int, c_void_p]),
     "pe_gemv_res_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "pe_gemv_swiglu_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "pe_dual_rmsnorm_add": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p]),

@@ -334,6 +334,75 @@ int pe_decode_layer(const pe_decode_layer_weights* w, const void* x, void* x_out
     return launch_decode_layer(a, (hipStream_t)stream);
 }
 
+int pe_gemv_w4(const void* x, long long ldx, int M, const pe_w4_weight* w, const void* bias, const void* res, long long ldr, void* out,
+               long long ldo, int swiglu, float norm_eps, void* stream) {
+    PE_REQUIRE(w, "pe_gemv_w4: null weight");
+    W4Problem p;
+    p.x = x; p.ldx = ldx; p.M = M; p.N = w->N; p.K = w->K; p.group = w->group;
+    p.codes = w->codes; p.scale = w->scale; p.zero = w->zero;
+    p.bias = bias; p.res = res; p.ldr = ldr; p.out = out; p.ldo = ldo;
+    p.swiglu = swiglu != 0; p.norm = norm_eps >= 0.f; p.eps = norm_eps;
+    return launch_gemv_w4(p, (hipStream_t)stream);
+}
+
+int pe_kv_append_e4m3(const pe_kv_cache* cache, const pe_kv_append_args* in, void* stream) {
+    PE_REQUIRE(cache && in, "pe_kv_append_e4m3: null argument");
+    KvAppend a;
+    a.kc = (uint8_t*)cache->k; a.vc = (uint8_t*)cache->v; a.ksc = cache->k_scale; a.vsc = cache->v_scale;
+    a.B = cache->batch; a.H = cache->n_kv; a.cap = cache->capacity; a.D = cache->head_dim;
+    a.q = (const bf16*)in->q; a.k = (const bf16*)in->k; a.v = (const bf16*)in->v;
+    for (int i = 0; i < 3; ++i) { a.qs[i] = in->q_strides[i]; a.ks[i] = in->k_strides[i]; a.vs[i] = in->v_strides[i]; }
+    a.q_out = (bf16*)in->q_out; a.cos = in->cos; a.sin = in->sin; a.table_rows = in->table_rows; a.table_f32 = in->table_f32;
+    a.positions = in->positions; a.start = in->start; a.T = in->T; a.n_q = in->n_q;
+    a.qk_blocks = a.v_blocks = 0;
+    return launch_kv_append(a, (hipStream_t)stream);
+}
+
+size_t pe_kv_attention_workspace_bytes(int batch, int n_kv, int T, int n_q, int head_dim, int capacity) {
+    return kv_attention_workspace_bytes(batch, n_kv, T, n_q, head_dim, capacity);
+}
+
+int pe_kv_attention_e4m3(const pe_kv_cache* cache, const void* q, const long long* q_strides, const int* start, const void* tree, int T, int n_q,
+                         float scale, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+    PE_REQUIRE(cache && q_strides, "pe_kv_attention_e4m3: null argument");
+    KvAttention a;
+    a.kc = (const uint8_t*)cache->k; a.vc = (const uint8_t*)cache->v; a.ksc = cache->k_scale; a.vsc = cache->v_scale;
+    a.B = cache->batch; a.H = cache->n_kv; a.cap = cache->capacity; a.D = cache->head_dim;
+    a.q = (const bf16*)q;
+    for (int i = 0; i < 3; ++i) a.qs[i] = q_strides[i];
+    a.out = (bf16*)out; a.start = start; a.tree = (const unsigned long long*)tree; a.T = T; a.n_q = n_q;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.splits = 1; a.part_o = a.part_ml = nullptr;
+    return launch_kv_attention(a, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+static LogitsArgs logits_args(const pe_logits_args* in, float* out) {
+    LogitsArgs a;
+    a.logits = in->logits; a.ld = in->ld; a.f32 = in->f32; a.rows = in->rows; a.V = in->vocab;
+    a.counts = (const short*)in->counts; a.ldc = in->ld_counts; a.penalties = in->penalties; a.ldp = in->ld_penalties;
+    a.bias = in->bias; a.ldb = in->ld_bias; a.allowed = (const uint32_t*)in->allowed; a.ldm = in->ld_allowed; a.out = out;
+    return a;
+}
+
+int pe_process_logits(const pe_logits_args* in, float* out, void* stream) {
+    PE_REQUIRE(in, "pe_process_logits: null argument");
+    return launch_process_logits(logits_args(in, out), (hipStream_t)stream);
+}
+
+size_t pe_select_token_workspace_bytes(int rows, int vocab) { return select_token_workspace_bytes(rows, vocab); }
+
+int pe_select_token(const pe_logits_args* in, int* token, int update_counts, int* out_ids, int* step, int max_steps, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+    PE_REQUIRE(in, "pe_select_token: null argument");
+    PE_REQUIRE(!update_counts || in->counts, "pe_select_token: no counts to update");
+    return launch_select_token(logits_args(in, nullptr), token, update_counts ? (short*)in->counts : nullptr, out_ids, step, max_steps, workspace,
+                               workspace_bytes, (hipStream_t)stream);
+}
+
+int pe_token_counts_add(void* counts, long long ld_counts, int rows, int vocab, const int* tokens, int n, int prompt, void* stream) {
+    return launch_token_counts_add((short*)counts, ld_counts, rows, vocab, tokens, n, prompt, (hipStream_t)stream);
+}
+
 int pe_decode_embed(const void* table, const int* token, void* x, int dim, int vocab, void* stream) {
     return launch_embed_row(table, token, x, dim, vocab, (hipStream_t)stream);
 }

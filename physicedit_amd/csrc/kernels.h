@@ -188,6 +188,75 @@ int launch_cfg_euler(const void* posi, const void* nega, const void* latents, vo
                      const void* input_latents = nullptr, const void* mask = nullptr, size_t plane = 0, float sigma = 0.f);
 
 // ---------------------------------------------------------------------------------------------
+// the low-bit decode step: 4-bit linears (w4.hip), the e4m3 key/value cache (kv_e4m3.hip), next-token scores (logits.hip)
+// ---------------------------------------------------------------------------------------------
+struct W4Problem {
+    const void* x;
+    long long ldx;
+    int M, N, K, group;
+    const void *codes, *scale, *zero;      // tiled layout of w4.hip; zero null: 8
+    const void *bias, *res;
+    long long ldr;
+    void* out;
+    long long ldo;
+    int swiglu, norm;                       // norm: the RMSNorm factor rsqrt(mean x^2 + eps)
+    float eps;
+};
+int launch_gemv_w4(const W4Problem& p, hipStream_t stream);
+
+struct KvAppend {
+    uint8_t *kc, *vc;
+    float *ksc, *vsc;
+    int B, H, cap, D;
+    const bf16 *q, *k, *v;                  // rows [b][t][head], strides in elements, channels contiguous
+    long long qs[3], ks[3], vs[3];
+    bf16* q_out;                            // [B][T][n_q][D]
+    const void *cos, *sin;                  // [table_rows][D], fp32 or bf16; null: no rotation
+    int table_rows, table_f32;
+    const int *positions, *start;           // [B][T] table rows (null: start + t), [B] cache rows before the new tokens
+    int T, n_q;
+    int qk_blocks, v_blocks;                // filled by the launch
+};
+int launch_kv_append(const KvAppend& a, hipStream_t stream);
+
+struct KvAttention {
+    const uint8_t *kc, *vc;
+    const float *ksc, *vsc;
+    int B, H, cap, D;
+    const bf16* q;
+    long long qs[3];
+    bf16* out;                              // [B][T][n_q][D]
+    const int* start;
+    const unsigned long long* tree;         // [B][T] or null: causal
+    int T, n_q;
+    float scale_log2;                       // softmax scale * log2(e)
+    int splits;                             // filled by the launch
+    float *part_o, *part_ml;
+};
+size_t kv_attention_workspace_bytes(int B, int H, int T, int n_q, int D, int cap);
+int launch_kv_attention(const KvAttention& a, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+struct LogitsArgs {
+    const void* logits;                     // [rows][V], row stride ld, fp32 or bf16
+    long long ld;
+    int f32, rows, V;
+    const short* counts;                    // [rows][V], row stride ldc
+    long long ldc;
+    const float* penalties;                 // [rows][3]: repetition, presence, frequency; ldp 0: one row for all
+    long long ldp;
+    const float* bias;                      // [V] (ldb 0) or [rows][V]
+    long long ldb;
+    const uint32_t* allowed;                // [words] (ldm 0) or [rows][words], bit set = allowed
+    long long ldm;
+    float* out;
+};
+int launch_process_logits(const LogitsArgs& a, hipStream_t stream);
+size_t select_token_workspace_bytes(int rows, int V);
+int launch_select_token(const LogitsArgs& a, int* token, short* count_into, int* out_ids, int* step, int max_steps, void* workspace,
+                        size_t workspace_bytes, hipStream_t stream);
+int launch_token_counts_add(short* counts, long long ldc, int rows, int V, const int* tokens, int n, int prompt, hipStream_t stream);
+
+// ---------------------------------------------------------------------------------------------
 // VAE (vae.hip): NHWC bf16 activations, channels padded to a multiple of 32
 // ---------------------------------------------------------------------------------------------
 int launch_conv_nhwc(const void* in, const void* w, const void* bias, const void* res, void* out, const void* zero,

@@ -1,0 +1,213 @@
+// Linears of a few rows with 4-bit weights and group scales (pe_gemv_w4).
+//
+//   y[m,n] = r[m] * sum_g s[n,g] * sum_{k in g} (c[n,k] - z[n,g]) x[m,k] + bias[n],     c, z in 0 .. 15, s bf16, g = 32, 64 or 128 inputs
+//   r[m] = rsqrt(mean_k x[m,k]^2 + eps) (an RMSNorm whose weight is folded into the weight's columns) or 1
+//   out = y + res,  or with the gated-MLP epilogue  out[m,f] = silu(y[m,f]) * y[m,F+f];  sums in fp32, one rounding to bf16 at the end.
+//
+// Every weight byte is used once, so the kernel is bound by HBM: N K / 2 bytes + N K / g * 2.5.  The products run on
+// v_mfma_f32_16x16x32_bf16 even for one row: with the weights as the 16-row operand an instruction takes 512 weights in 16 cycles of its
+// SIMD, four times what HBM delivers to a CU, and up to 16 rows of x cost what one does.
+// A code becomes a bf16 by ORing it into the mantissa of 128.0: (u >> 4 i) & 0x000f000f | 0x43004300 is the pair 128 + c, so two weights cost
+// two instructions (a shift and an and-or).  The offset and the zero point leave through the row sum of x over the group,
+//   sum (c - z) x = sum (128 + c) x - (128 + z) sum x,
+// which one more MFMA per 32 inputs (ones as the weights) gives every lane for the rows it holds; products of two bf16 are exact in
+// fp32, so this costs about 2^-24 * 136 * sum |x| of a group, far below the output's bf16 rounding.  r comes the same way: x as BOTH
+// operands leaves sum x^2 on the diagonal.
+//
+// Layout of the codes: tiles of 16 outputs x 128 inputs, 1 KiB, [N/16][K/128][lane][step]: the lane's four words are its A fragments of the
+// four 32-input steps (output lane & 15, inputs 32 step + 8 (lane >> 4) + e, element e in nibble (e >> 1) + 4 (e & 1)), one coalesced 16-byte load
+// per lane and tile.  Scales and zero points are [N/16][groups][16].  N is padded to 16 with scales of 0, K to 128 (x is read as 0 there).
+//
+// A work-group of W waves takes R tiles of 16 outputs; its waves take turns at the 128-input chunks and join their fp32 sums in LDS in a
+// fixed order: results do not depend on scheduling.  Lanes of rows >= M read row M - 1 again: their columns are never stored.
+#include "common.h"
+#include "kernels.h"
+
+namespace pe {
+
+struct W4Args {
+    const bf16* x;
+    const u32x4* codes;
+    const bf16* scale;
+    const uint8_t* zero;      // null: 8
+    const bf16* bias;
+    const bf16* res;
+    bf16* out;
+    long long ldx, ldr, ldo;
+    int M, N, K, KC, G;       // KC = chunks of 128 inputs, G = groups (K padded to 128)
+    int pair_tiles;           // gated epilogue: tile of the up row = tile of the gate row + pair_tiles
+    float eps;                // >= 0: RMSNorm factor
+    int norm;
+};
+
+PE_DEV bf16x8 w4_fragment(uint32_t u) {
+    u32x4 f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = ((u >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    return __builtin_bit_cast(bf16x8, f);
+}
+
+// MT: tiles of 16 rows of x.  R: weight tiles of a work-group.  GS: 32-input steps of a group (1, 2, 4).
+template <int MT, int R, int W, int GS, bool SWIGLU>
+__global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
+    __shared__ f32x4 part[W][R][64];
+    __shared__ float sq[W][MT * 16];
+    const int lane = lane_id(), w = wave_id(), j = lane >> 4, c = lane & 15;
+    const int ntiles = (a.N + 15) >> 4;
+    int tile[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int t = SWIGLU ? (int)blockIdx.x * (R / 2) + (r >> 1) : (int)blockIdx.x * R + r;
+        tile[r] = SWIGLU ? min(t, a.pair_tiles - 1) + (r & 1) * a.pair_tiles : min(t, ntiles - 1);
+    }
+    const bf16* xrow[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) xrow[mt] = a.x + (size_t)min(mt * 16 + c, a.M - 1) * a.ldx + 8 * j;
+
+    f32x4 acc[R][MT] = {};
+    f32x4 gram[MT] = {};
+    bf16x8 ones;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ones[e] = (bf16)1.0f;
+
+    for (int kc = w; kc < a.KC; kc += W) {
+        u32x4 wq[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) wq[r] = __builtin_nontemporal_load(a.codes + ((size_t)tile[r] * a.KC + kc) * 64 + lane);
+        bf16x8 b[MT][4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int k = kc * 128 + 32 * s;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) b[mt][s] = k < a.K ? *(const bf16x8*)(xrow[mt] + k) : bf16x8{};
+        }
+        if (a.norm) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) gram[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[mt][s], b[mt][s], gram[mt], 0, 0, 0);
+        }
+#pragma unroll
+        for (int g = 0; g < 4 / GS; ++g) {
+            const int grp = kc * (4 / GS) + g;
+            f32x4 sum[R][MT] = {}, sx[MT] = {};
+#pragma unroll
+            for (int s = g * GS; s < (g + 1) * GS; ++s) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) sx[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, b[mt][s], sx[mt], 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const bf16x8 f = w4_fragment(wq[r][s]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) sum[r][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, b[mt][s], sum[r][mt], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const size_t at = ((size_t)tile[r] * a.G + grp) * 16 + 4 * j;
+                const bf16x4 sc = *(const bf16x4*)(a.scale + at);
+                const uint32_t z = a.zero ? *(const uint32_t*)(a.zero + at) : 0x08080808u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float off = -(128.0f + (float)((z >> (8 * i)) & 0xff));
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+                        acc[r][mt][i] = __builtin_fmaf((float)sc[i], __builtin_fmaf(off, sx[mt][i], sum[r][mt][i]), acc[r][mt][i]);
+                }
+            }
+        }
+    }
+
+    if (a.norm) {           // the diagonal: row 4 j + i == column c
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (4 * j + i == c) sq[w][mt * 16 + c] = gram[mt][i];
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) part[w][r][lane] = acc[r][mt];
+        __syncthreads();
+        constexpr int OUT = SWIGLU ? R / 2 : R;
+        for (int o = w; o < OUT; o += W) {
+            const int m = mt * 16 + c;
+            float rs = 1.0f;
+            if (a.norm) {
+                float t = 0.f;
+#pragma unroll
+                for (int v = 0; v < W; ++v) t += sq[v][m];
+                rs = rsqrtf(t / (float)a.K + a.eps);
+            }
+            f32x4 y[2] = {};
+#pragma unroll
+            for (int p = 0; p < (SWIGLU ? 2 : 1); ++p) {
+#pragma unroll
+                for (int v = 0; v < W; ++v) y[p] += part[v][SWIGLU ? 2 * o + p : o][lane];
+            }
+            const int t = (int)blockIdx.x * OUT + o;
+            const int n0 = t * 16 + 4 * j, cols = SWIGLU ? a.N / 2 : a.N;
+            if (m < a.M && n0 < cols) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int n = n0 + i;
+                    if (n >= cols) break;
+                    float v = y[0][i] * rs + (a.bias ? (float)a.bias[n] : 0.f);
+                    if (SWIGLU) {
+                        const float u = y[1][i] * rs + (a.bias ? (float)a.bias[cols + n] : 0.f);
+                        v = v * sigmoidf_(v) * u;
+                    }
+                    if (a.res) v += (float)a.res[(size_t)m * a.ldr + n];
+                    a.out[(size_t)m * a.ldo + n] = (bf16)v;
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <int MT, int R, int W, bool SWIGLU>
+static void w4_launch(const W4Args& a, int gs, hipStream_t stream) {
+    const int tiles = SWIGLU ? a.pair_tiles : (a.N + 15) / 16, per = SWIGLU ? R / 2 : R;
+    const dim3 grid((tiles + per - 1) / per), block(W * 64);
+    if (gs == 1) hipLaunchKernelGGL((gemv_w4_kernel<MT, R, W, 1, SWIGLU>), grid, block, 0, stream, a);
+    else if (gs == 2) hipLaunchKernelGGL((gemv_w4_kernel<MT, R, W, 2, SWIGLU>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((gemv_w4_kernel<MT, R, W, 4, SWIGLU>), grid, block, 0, stream, a);
+}
+
+int launch_gemv_w4(const W4Problem& p, hipStream_t stream) {
+    PE_REQUIRE(p.x && p.codes && p.scale && p.out, "gemv_w4: null pointer");
+    PE_REQUIRE(p.group == 32 || p.group == 64 || p.group == 128, "gemv_w4: group of %d inputs (32, 64 or 128)", p.group);
+    PE_REQUIRE(p.M >= 1 && p.M <= 64, "gemv_w4: M=%d rows (1 ... 64; more rows are a matrix product)", p.M);
+    PE_REQUIRE(p.N >= 1 && p.K >= p.group && p.K % p.group == 0, "gemv_w4: N=%d K=%d (K must be a multiple of the group %d)", p.N, p.K, p.group);
+    PE_REQUIRE(p.N <= (1 << 26) && p.K <= (1 << 22), "gemv_w4: N=%d K=%d out of range", p.N, p.K);
+    PE_REQUIRE(p.ldx >= p.K && p.ldx % 8 == 0 && ((uintptr_t)p.x & 15) == 0, "gemv_w4: rows of x must be 16-byte aligned (ldx=%lld)", p.ldx);
+    PE_REQUIRE(((uintptr_t)p.codes & 15) == 0 && ((uintptr_t)p.scale & 15) == 0 && ((uintptr_t)p.zero & 15) == 0, "gemv_w4: unaligned weight");
+    const int cols = p.swiglu ? p.N / 2 : p.N;
+    PE_REQUIRE(!p.swiglu || p.N % 32 == 0, "gemv_w4: the gated epilogue needs a multiple of 16 gate and up rows (N=%d)", p.N);
+    PE_REQUIRE(!(p.swiglu && p.res), "gemv_w4: no residual with the gated epilogue");
+    PE_REQUIRE(p.ldo >= cols && (!p.res || p.ldr >= cols), "gemv_w4: row stride below the %d columns", cols);
+    PE_REQUIRE(!p.norm || p.eps >= 0.f, "gemv_w4: negative eps");
+    W4Args a;
+    a.x = (const bf16*)p.x; a.codes = (const u32x4*)p.codes; a.scale = (const bf16*)p.scale; a.zero = (const uint8_t*)p.zero;
+    a.bias = (const bf16*)p.bias; a.res = (const bf16*)p.res; a.out = (bf16*)p.out;
+    a.ldx = p.ldx; a.ldr = p.ldr; a.ldo = p.ldo;
+    a.M = p.M; a.N = p.N; a.K = p.K; a.KC = (p.K + 127) / 128; a.G = a.KC * (128 / p.group);
+    a.pair_tiles = p.swiglu ? p.N / 32 : 0;
+    a.norm = p.norm; a.eps = p.eps;
+    const int gs = p.group / 32;
+    const int mt = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
+    if (p.swiglu) {
+        if (mt == 1) w4_launch<1, 2, 4, true>(a, gs, stream);
+        else if (mt == 2) w4_launch<2, 2, 4, true>(a, gs, stream);
+        else w4_launch<4, 2, 4, true>(a, gs, stream);
+    } else {
+        if (mt == 1) w4_launch<1, 1, 8, false>(a, gs, stream);
+        else if (mt == 2) w4_launch<2, 1, 8, false>(a, gs, stream);
+        else w4_launch<4, 1, 8, false>(a, gs, stream);
+    }
+    return check_launch("gemv_w4_kernel");
+}
+
+}  // namespace pe

@@ -497,3 +497,290 @@ def sdpa_heads64(q: torch.Tensor, kv: torch.Tensor, heads: int) -> torch.Tensor:
     out = torch.empty_like(q)
     check(lib().pe_sdpa_heads64(q.data_ptr(), kv.data_ptr(), out.data_ptr(), nq, nk, heads, 64 ** -0.5, stream_ptr()), "pe_sdpa_heads64")
     return out
+
+
+# ---- the low-bit decode step: 4-bit linears, the e4m3 key/value cache, next-token scores (include/physicedit_amd.h) -----------------
+def _here(*named: Tuple[Optional[torch.Tensor], str]) -> torch.device:
+    """the one device of the given tensors, which has to be the current one: the launch goes to the current stream"""
+    dev = named[0][0].device
+    for t, name in named:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name}: expected a CUDA/HIP tensor (physicedit_amd has no CPU path)")
+        if t.device != dev or t.device.index != torch.cuda.current_device():
+            raise ValueError(f"{name}: on {t.device}, but the current device is cuda:{torch.cuda.current_device()} (torch.cuda.device(...))")
+    return dev
+
+
+def _want(t: torch.Tensor, name: str, dtype: torch.dtype, shape: Tuple[int, ...]) -> torch.Tensor:
+    """a contiguous tensor of exactly this type and shape"""
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return t
+
+
+class W4Weight:
+    """A linear's weight [N, K] as 4-bit codes with a scale (and a zero point) per output and `group` inputs, in the layout of pe_gemv_w4
+    (include/physicedit_amd.h, pe_w4_weight).  Made by pack_w4 / quantize_w4."""
+
+    def __init__(self, codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor], N: int, K: int, group: int):
+        self.codes, self.scale, self.zero, self.N, self.K, self.group = codes, scale, zero, N, K, group
+        self._c = _lib.W4Weight(codes.data_ptr(), scale.data_ptr(), _ptr(zero), N, K, group)
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.codes, self.scale, self.zero) if t is not None)
+
+
+def pack_w4(codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor] = None, group: int = 128) -> W4Weight:
+    """codes uint8 [N, K/2] (input 2i in the low nibble of byte i), scale bf16 [N, K/group], zero uint8 [N, K/group] in 0 ... 15 or None (8):
+    weight = scale * (code - zero).  Lays them out once for gemv_w4."""
+    dev = _here((codes, "codes"), (scale, "scale"), (zero, "zero"))
+    if codes.dim() != 2 or group not in (32, 64, 128):
+        raise ValueError(f"pack_w4: codes [N, K/2] and a group of 32, 64 or 128, got {tuple(codes.shape)} and {group}")
+    N, K = codes.shape[0], codes.shape[1] * 2
+    if N < 1 or K < group or K % group:
+        raise ValueError(f"pack_w4: K={K} must be a multiple of the group {group}")
+    _want(codes, "codes", torch.uint8, (N, K // 2)), _want(scale, "scale", BF, (N, K // group))
+    if zero is not None:
+        _want(zero, "zero", torch.uint8, (N, K // group))
+    tiles, chunks = (N + 15) // 16, (K + 127) // 128
+    full = torch.zeros((tiles * 16, chunks * 64), dtype=torch.uint8, device=dev)
+    full[:N, :K // 2] = codes
+    # byte (step s, lane group j, i) = elements 2 i, 2 i + 1 of the lane's eight: nibbles i and 4 + i of its word
+    b = full.view(tiles, 16, chunks, 4, 4, 4).permute(0, 2, 4, 1, 3, 5)               # tile, chunk, j, output, s, i
+    low, high = b & 15, b >> 4
+    words = torch.empty((tiles, chunks, 4, 16, 4, 4), dtype=torch.uint8, device=dev)   # bytes of the word: nibble pairs (0,1) (2,3) | (4,5) (6,7)
+    words[..., 0], words[..., 1] = low[..., 0] | (low[..., 1] << 4), low[..., 2] | (low[..., 3] << 4)
+    words[..., 2], words[..., 3] = high[..., 0] | (high[..., 1] << 4), high[..., 2] | (high[..., 3] << 4)
+
+    def per_group(t, fill):
+        padded = torch.full((tiles * 16, chunks * (128 // group)), fill, dtype=t.dtype, device=dev)
+        padded[:N, :K // group] = t
+        return padded.view(tiles, 16, -1).transpose(1, 2).contiguous()
+
+    return W4Weight(words.view(tiles, chunks, 64, 16), per_group(scale, 0), None if zero is None else per_group(zero & 15, 8), N, K, group)
+
+
+def quantize_w4(w: torch.Tensor, group: int = 128, zero_point: bool = True, norm_w: Optional[torch.Tensor] = None) -> W4Weight:
+    """Round-to-nearest 4-bit form of a bf16 weight [N, K]: per output and group, zero_point: scale = (max(w, 0) - min(w, 0)) / 15 and
+    zero = round(-min / scale), else scale = max|w| / 7 and zero = 8.  norm_w [K]: the weight of an RMSNorm in front of the linear, folded
+    into the columns first (gemv_w4(norm_eps=...) applies the rest of the norm)."""
+    _chk(w, "w"), _here((w, "w"), (norm_w, "norm_w"))
+    N, K = w.shape
+    if group not in (32, 64, 128) or K % group or K < group:
+        raise ValueError(f"quantize_w4: K={K} must be a multiple of the group {group} (32, 64 or 128)")
+    codes, scale = torch.empty((N, K // 2), dtype=torch.uint8, device=w.device), torch.empty((N, K // group), dtype=BF, device=w.device)
+    zero = torch.empty((N, K // group), dtype=torch.uint8, device=w.device) if zero_point else None
+    for lo in range(0, N, 16384):                                    # in slices: the fp32 copies of a vocabulary are large
+        x = w[lo:lo + 16384].float()
+        if norm_w is not None:
+            x = x * norm_w.float()
+        x = x.view(x.shape[0], -1, group)
+        if zero_point:
+            top, low = x.amax(-1).clamp_min(0), x.amin(-1).clamp_max(0)
+            s = ((top - low) / 15).to(BF)
+            z = torch.where(s > 0, torch.round(-low / s.float()), torch.zeros_like(low)).clamp_(0, 15)
+            zero[lo:lo + 16384] = z.to(torch.uint8)
+        else:
+            s = (x.abs().amax(-1) / 7).to(BF)
+            z = torch.full_like(s, 8, dtype=torch.float32)
+        q = torch.where(s[..., None] > 0, torch.round(x / s.float()[..., None]), torch.zeros_like(x)) + z[..., None]
+        q = q.clamp_(0, 15).to(torch.uint8).flatten(1)
+        codes[lo:lo + 16384], scale[lo:lo + 16384] = q[:, 0::2] | (q[:, 1::2] << 4), s
+    return pack_w4(codes, scale, zero, group)
+
+
+def gemv_w4(x: torch.Tensor, w: W4Weight, bias: Optional[torch.Tensor] = None, res: Optional[torch.Tensor] = None, epilogue: str = "bias",
+            norm_eps: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x [M, K] or [K] (M <= 64 rows; a row stride is fine) @ w.T + bias + res -> [M, N] or [N], one rounding.  epilogue="swiglu": w holds the gate
+    rows, then as many up rows (a multiple of 16): silu(gate) * up.  norm_eps: x is RMS-normalised (its norm weight folded into w)."""
+    if epilogue not in ("bias", "swiglu"):
+        raise ValueError(f"gemv_w4: epilogue {epilogue!r} ('bias' or 'swiglu')")
+    if norm_eps is not None and not norm_eps >= 0:
+        raise ValueError(f"gemv_w4: norm_eps={norm_eps}")
+    dev = _here((x, "x"), (w.codes, "w"), (bias, "bias"), (res, "res"), (out, "out"))
+    one = x.dim() == 1
+    rows = x.unsqueeze(0) if one else x
+    if rows.dim() != 2 or rows.dtype != BF or rows.shape[1] != w.K or rows.stride(1) != 1:
+        raise ValueError(f"gemv_w4: expected bf16 rows of {w.K} contiguous values, got {x.dtype} {tuple(x.shape)}")
+    M = rows.shape[0]
+    swiglu = epilogue == "swiglu"
+    cols = w.N // 2 if swiglu else w.N
+    shape = (cols,) if one else (M, cols)
+    if bias is not None:
+        _want(bias, "bias", BF, (w.N,))
+    if res is not None:
+        _want(res, "res", BF, shape)
+    out = torch.empty(shape, dtype=BF, device=dev) if out is None else _want(out, "out", BF, shape)
+    check(lib().pe_gemv_w4(rows.data_ptr(), rows.stride(0) if M > 1 else w.K, M, C.byref(w._c), _ptr(bias), _ptr(res), cols, out.data_ptr(), cols,
+                           int(swiglu), -1.0 if norm_eps is None else float(norm_eps), stream_ptr()), "pe_gemv_w4")
+    return out
+
+
+class KVCacheE4M3:
+    """The keys and values of one layer as e4m3 codes with a scale per (sequence, token, kv head), zero at first.  capacity: a multiple of 64.
+    Views of the buffers: k [batch, n_kv, capacity, head_dim], v [batch, n_kv, capacity/64, 64, head_dim] (stored transposed in blocks of
+    64 tokens), k_scale / v_scale [batch, n_kv, capacity]; value = code * scale."""
+
+    def __init__(self, batch: int, n_kv: int, capacity: int, head_dim: int = 128, device="cuda"):
+        if batch < 1 or n_kv < 1 or capacity < 64 or capacity % 64 or capacity > 1 << 30 or head_dim not in (64, 128):
+            raise ValueError(f"KVCacheE4M3: batch={batch} n_kv={n_kv} capacity={capacity} (a multiple of 64) head_dim={head_dim} (64 or 128)")
+        self.batch, self.n_kv, self.capacity, self.head_dim = batch, n_kv, capacity, head_dim
+        self._k = torch.zeros((batch, n_kv, capacity, head_dim), dtype=torch.uint8, device=device)
+        self._v = torch.zeros((batch, n_kv, capacity // 64, head_dim, 64), dtype=torch.uint8, device=device)
+        self.k_scale = torch.zeros((batch, n_kv, capacity), dtype=torch.float32, device=device)
+        self.v_scale = torch.zeros_like(self.k_scale)
+        self._c = _lib.KvCache(self._k.data_ptr(), self._v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), batch, n_kv, capacity, head_dim)
+        self.k = self._k.view(F8)
+        self.v = self._v.view(F8).transpose(3, 4)
+
+    def start(self, start: torch.Tensor) -> torch.Tensor:
+        return _want(start, "start", torch.int32, (self.batch,))
+
+
+def _rows3(t: torch.Tensor, name: str, batch: int, T: int, heads: int, D: int):
+    """strides (batch, token, head) of a bf16 [batch, T, heads, D] tensor with contiguous channels"""
+    if t.dtype != BF or tuple(t.shape) != (batch, T, heads, D) or t.stride(3) != 1:
+        raise ValueError(f"{name}: expected bf16 [{batch}, {T}, {heads}, {D}] with contiguous channels, got {t.dtype} {tuple(t.shape)}")
+    st = [t.stride(i) if t.shape[i] > 1 else D for i in range(3)]          # the stride of a single entry is never used
+    if any(s % 8 for s in st) or t.data_ptr() % 16:
+        raise ValueError(f"{name}: rows must be 16-byte aligned (strides {tuple(t.stride())})")
+    return (C.c_longlong * 3)(*st)
+
+
+def kv_append_e4m3(cache: KVCacheE4M3, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, q: Optional[torch.Tensor] = None,
+                   cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """k, v [batch, T, n_kv, D] (any strides of whole 16 bytes) into rows start[b] ... start[b] + T - 1 (int32 [batch], device) of the cache.  cos, sin
+    [rows, D] (bf16 or fp32): k -- and q [batch, T, n_q, D], returned rotated, contiguous -- are rotated with table row positions[b, t] (int32;
+    default start[b] + t) first.  Rows past the capacity and sequences with start < 0 are not written (their q comes back zero)."""
+    dev = _here((cache.k_scale, "cache"), (k, "k"), (v, "v"), (start, "start"), (q, "q"), (cos, "cos"), (sin, "sin"), (positions, "positions"), (out, "out"))
+    if k.dim() != 4:
+        raise ValueError(f"k: expected [batch, T, n_kv, D], got {tuple(k.shape)}")
+    B, T, H, D = cache.batch, k.shape[1], cache.n_kv, cache.head_dim
+    a = _lib.KvAppendArgs(k=k.data_ptr(), v=v.data_ptr(), k_strides=_rows3(k, "k", B, T, H, D), v_strides=_rows3(v, "v", B, T, H, D), T=T,
+                          start=cache.start(start).data_ptr())
+    if (cos is None) != (sin is None) or (cos is None and (q is not None or positions is not None)):
+        raise ValueError("kv_append_e4m3: q and positions need cos and sin, which come together")
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape[1] != D or cos.dtype not in (BF, torch.float32) or not cos.is_contiguous():
+            raise ValueError(f"cos: expected contiguous bf16 or fp32 [rows, {D}], got {cos.dtype} {tuple(cos.shape)}")
+        _want(sin, "sin", cos.dtype, cos.shape)
+        a.cos, a.sin, a.table_rows, a.table_f32 = cos.data_ptr(), sin.data_ptr(), cos.shape[0], int(cos.dtype == torch.float32)
+        if positions is not None:
+            a.positions = _want(positions, "positions", torch.int32, (B, T)).data_ptr()
+    if q is not None:
+        if q.dim() != 4:
+            raise ValueError(f"q: expected [batch, T, n_q, D], got {tuple(q.shape)}")
+        a.n_q = q.shape[2]
+        a.q, a.q_strides = q.data_ptr(), _rows3(q, "q", B, T, a.n_q, D)
+        out = torch.empty((B, T, a.n_q, D), dtype=BF, device=dev) if out is None else _want(out, "out", BF, (B, T, a.n_q, D))
+        a.q_out = out.data_ptr()
+    check(lib().pe_kv_append_e4m3(C.byref(cache._c), C.byref(a), stream_ptr()), "pe_kv_append_e4m3")
+    return out if q is not None else None
+
+
+def kv_attention_workspace(cache: KVCacheE4M3, T: int, n_q: int) -> torch.Tensor:
+    """scratch of kv_attention_e4m3 for calls that want to keep one (one per stream)"""
+    return torch.empty((lib().pe_kv_attention_workspace_bytes(cache.batch, cache.n_kv, T, n_q, cache.head_dim, cache.capacity),),
+                       dtype=torch.uint8, device=cache.k_scale.device)
+
+
+def kv_attention_e4m3(q: torch.Tensor, cache: KVCacheE4M3, start: torch.Tensor, tree: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                      out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the T <= 64 newest tokens, appended at rows start[b] + t: q [batch, T, n_q, D] -> [batch, T, n_q * D].  Token t sees the cache rows
+    below start[b] and new token j where bit j of tree[b, t] (int64) is set; tree None: causal.  scale: default 1 / sqrt(D).  A query that sees
+    nothing gives zeros."""
+    dev = _here((cache.k_scale, "cache"), (q, "q"), (start, "start"), (tree, "tree"), (out, "out"), (workspace, "workspace"))
+    if q.dim() != 4:
+        raise ValueError(f"q: expected [batch, T, n_q, D], got {tuple(q.shape)}")
+    B, T, n_q, D = cache.batch, q.shape[1], q.shape[2], cache.head_dim
+    strides = _rows3(q, "q", B, T, n_q, D)
+    if not 1 <= T <= 64 or n_q % cache.n_kv:
+        raise ValueError(f"kv_attention_e4m3: {T} new tokens (1 ... 64), {n_q} query heads over {cache.n_kv} kv heads")
+    if tree is not None:
+        _want(tree, "tree", torch.int64, (B, T))
+    out = torch.empty((B, T, n_q * D), dtype=BF, device=dev) if out is None else _want(out, "out", BF, (B, T, n_q * D))
+    ws = kv_attention_workspace(cache, T, n_q) if workspace is None else workspace
+    check(lib().pe_kv_attention_e4m3(C.byref(cache._c), q.data_ptr(), strides, cache.start(start).data_ptr(), _ptr(tree), T, n_q,
+                                     1.0 / math.sqrt(D) if scale is None else float(scale), out.data_ptr(), ws.data_ptr(),
+                                     ws.numel() * ws.element_size(), stream_ptr()), "pe_kv_attention_e4m3")
+    return out
+
+
+def _logits_args(logits, counts, penalties, bias, allowed):
+    dev = _here((logits, "logits"), (counts, "counts"), (penalties, "penalties"), (bias, "bias"), (allowed, "allowed"))
+    if logits.dim() != 2 or logits.dtype not in (BF, torch.float32) or logits.stride(1) != 1 or logits.numel() == 0:
+        raise ValueError(f"logits: expected bf16 or fp32 [rows, vocab] with contiguous rows, got {logits.dtype} {tuple(logits.shape)}")
+    R, V = logits.shape
+    a = _lib.LogitsArgs(logits=logits.data_ptr(), ld=logits.stride(0) if R > 1 else V, f32=int(logits.dtype == torch.float32), rows=R, vocab=V)
+
+    def table(t, name, dtype, n):
+        if t.dim() == 1 and name != "counts":
+            _want(t, name, dtype, (n,))
+            return 0
+        _want(t, name, dtype, (R, n))
+        return n
+    if penalties is not None and counts is None:
+        raise ValueError("penalties: they need the counts")
+    if counts is not None:
+        a.counts, a.ld_counts = counts.data_ptr(), table(counts, "counts", torch.int16, V)
+    if penalties is not None:
+        a.penalties, a.ld_penalties = penalties.data_ptr(), table(penalties, "penalties", torch.float32, 3)
+    if bias is not None:
+        a.bias, a.ld_bias = bias.data_ptr(), table(bias, "bias", torch.float32, V)
+    if allowed is not None:
+        a.allowed, a.ld_allowed = allowed.data_ptr(), table(allowed, "allowed", torch.int32, (V + 31) // 32)
+    return a, R, V, dev
+
+
+def process_logits(logits: torch.Tensor, counts: Optional[torch.Tensor] = None, penalties: Optional[torch.Tensor] = None,
+                   bias: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """logits [rows, vocab] (bf16 or fp32) -> fp32 scores with repetition / presence / frequency penalties, a bias and a mask, in this order.
+    counts int16 [rows, vocab]: bit 15 (the value is negative) = the prompt holds the token, the rest = how often it was generated (token_counts_add
+    keeps them); penalties fp32 [rows, 3] or [3]: repetition (divides positive, multiplies other scores of seen tokens), presence, frequency; bias fp32
+    [vocab] or [rows, vocab]; allowed int32 [rows, ceil(vocab / 32)] or [ceil(vocab / 32)]: token v is bit v % 32 of word v / 32, clear = -inf."""
+    a, R, V, dev = _logits_args(logits, counts, penalties, bias, allowed)
+    out = torch.empty((R, V), dtype=torch.float32, device=dev) if out is None else _want(out, "out", torch.float32, (R, V))
+    if out.device != dev:
+        raise ValueError(f"out: on {out.device}, the logits on {dev}")
+    check(lib().pe_process_logits(C.byref(a), out.data_ptr(), stream_ptr()), "pe_process_logits")
+    return out
+
+
+def select_token(logits: torch.Tensor, counts: Optional[torch.Tensor] = None, penalties: Optional[torch.Tensor] = None,
+                 bias: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None, update_counts: bool = False,
+                 out: Optional[torch.Tensor] = None, out_ids: Optional[torch.Tensor] = None, step: Optional[torch.Tensor] = None,
+                 workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The greedy choice among process_logits' scores, without writing them: int32 [rows], the first maximum (NaN never wins), -1 where everything
+    is -inf.  update_counts: counts[row, token] += 1.  step / out_ids (int32, one row): decode_argmax's device-side counter and token list."""
+    a, R, V, dev = _logits_args(logits, counts, penalties, bias, allowed)
+    if update_counts and counts is None:
+        raise ValueError("select_token: update_counts without counts")
+    out = torch.empty((R,), dtype=torch.int32, device=dev) if out is None else _want(out, "out", torch.int32, (R,))
+    if (step is None) != (out_ids is None) or (step is not None and (R != 1 or step.numel() != 1 or out_ids.numel() < 1)):
+        raise ValueError("select_token: step and out_ids come together, for one row")
+    if step is not None:
+        _chk_i32(step, "step"), _chk_i32(out_ids, "out_ids")
+    if workspace is None:
+        workspace = torch.empty((lib().pe_select_token_workspace_bytes(R, V),), dtype=torch.uint8, device=dev)
+    _here((logits, "logits"), (out, "out"), (out_ids, "out_ids"), (step, "step"), (workspace, "workspace"))
+    check(lib().pe_select_token(C.byref(a), out.data_ptr(), int(update_counts), _ptr(out_ids), _ptr(step), 0 if out_ids is None else out_ids.numel(),
+                                workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream_ptr()), "pe_select_token")
+    return out
+
+
+def token_counts_add(counts: torch.Tensor, tokens: torch.Tensor, prompt: bool = False) -> torch.Tensor:
+    """counts int16 [rows, vocab] of process_logits, in place: every id of tokens int32 [rows, n] counts one more (up to 32767), or with prompt=True
+    is marked as part of the prompt.  Ids outside the vocabulary (padding: -1) are skipped."""
+    _here((counts, "counts"), (tokens, "tokens"))
+    if counts.dim() != 2 or counts.dtype != torch.int16 or not counts.is_contiguous() or counts.numel() == 0:
+        raise ValueError(f"counts: expected a contiguous int16 [rows, vocab], got {counts.dtype} {tuple(counts.shape)}")
+    R, V = counts.shape
+    if tokens.dim() != 2 or tokens.shape[1] < 1:
+        raise ValueError(f"tokens: expected int32 [{R}, n], got {tuple(tokens.shape)}")
+    _want(tokens, "tokens", torch.int32, (R, tokens.shape[1]))
+    check(lib().pe_token_counts_add(counts.data_ptr(), V, R, V, tokens.data_ptr(), tokens.shape[1], int(prompt), stream_ptr()), "pe_token_counts_add")
+    return counts
