@@ -303,9 +303,10 @@ int pe_decode_argmax(const void* logits, int vocab, int* token, int* out_ids, in
  * (32, 64 or 128; K a multiple of it), laid out once (ops.pack_w4 / ops.quantize_w4 write it):
  *   codes  [ceil(N/16)][ceil(K/128)][64][4] words, 16-byte aligned: word s of lane l holds output l % 16 of the tile, inputs 32 s + 8 (l / 16) + e of the
  *          chunk, element e in nibble e / 2 + 4 (e % 2);
- *   scale  [ceil(N/16)][128 / group * ceil(K/128)][16] bf16, 0 for outputs >= N and inputs >= K;  zero: the same shape in bytes, NULL = 8 everywhere. */
+ *   scale  [ceil(N/16)][128 / group * ceil(K/128)][16] words, 16-byte aligned: the scale's bf16 in the low half, the bf16 of -(128 + zero) in the high
+ *          half; words of outputs >= N and of groups beyond K are 0. */
 typedef struct pe_w4_weight {
-    const void *codes, *scale, *zero;
+    const void *codes, *scale;
     int N, K, group;
 } pe_w4_weight;
 /* out[M, N] = r * (x @ W^T) + bias + res for 1 ... 64 rows x [M,K] bf16 (finite values; row stride ldx, a multiple of 8; 16-byte aligned).  norm_eps >= 0:

@@ -54,7 +54,7 @@ class DecodeLayerWeights(C.Structure):
 
 class W4Weight(C.Structure):
     """pe_w4_weight"""
-    _fields_ = [("codes", c_void_p), ("scale", c_void_p), ("zero", c_void_p), ("N", c_int), ("K", c_int), ("group", c_int)]
+    _fields_ = [("codes", c_void_p), ("scale", c_void_p), ("N", c_int), ("K", c_int), ("group", c_int)]
 
 
 class KvCache(C.Structure):

@@ -339,7 +339,7 @@ int pe_gemv_w4(const void* x, long long ldx, int M, const pe_w4_weight* w, const
     PE_REQUIRE(w, "pe_gemv_w4: null weight");
     W4Problem p;
     p.x = x; p.ldx = ldx; p.M = M; p.N = w->N; p.K = w->K; p.group = w->group;
-    p.codes = w->codes; p.scale = w->scale; p.zero = w->zero;
+    p.codes = w->codes; p.scale = w->scale;
     p.bias = bias; p.res = res; p.ldr = ldr; p.out = out; p.ldo = ldo;
     p.swiglu = swiglu != 0; p.norm = norm_eps >= 0.f; p.eps = norm_eps;
     return launch_gemv_w4(p, (hipStream_t)stream);

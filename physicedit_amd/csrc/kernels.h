@@ -194,7 +194,7 @@ struct W4Problem {
     const void* x;
     long long ldx;
     int M, N, K, group;
-    const void *codes, *scale, *zero;      // tiled layout of w4.hip; zero null: 8
+    const void *codes, *scale;              // tiled layout of w4.hip
     const void *bias, *res;
     long long ldr;
     void* out;

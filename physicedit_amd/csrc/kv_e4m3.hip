@@ -204,12 +204,14 @@ PE_DEV bf16x8 codes8(uint32_t a, uint32_t b) {
     return bf16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
 }
 
-template <int D, int RT>
-__global__ void __launch_bounds__(256) kv_attention_kernel(KvAttention a) {
+// WR row tiles x WK shares of the cache's blocks = the waves of a work-group: with one row tile (decode: T * n_q / H <= 16 rows) all waves share its
+// blocks and are joined in LDS; with more rows a wave takes 16 of them and the waves read the same blocks through the cache.
+template <int D, int WR, int WK>
+__global__ void __launch_bounds__(WR * WK * 64) kv_attention_kernel(KvAttention a) {
     constexpr int DT = D / 16, KS = D / 32;
-    __shared__ float lds_o[4][DT][64][4];
-    __shared__ float lds_m[4][16], lds_l[4][16];
-    const int lane = lane_id(), w = wave_id(), j = lane >> 4, c = lane & 15;
+    __shared__ float lds_o[WK > 1 ? WR * WK : 1][WK > 1 ? DT : 1][64][4];
+    __shared__ float lds_m[WR * WK][16], lds_l[WR * WK][16];
+    const int lane = lane_id(), w = wave_id(), wr = w % WR, wk = w / WR, j = lane >> 4, c = lane & 15;
     const int split = (int)blockIdx.x, b = (int)blockIdx.z;
     const int hk = (int)blockIdx.y % a.H, rb = (int)blockIdx.y / a.H;
     const int G = a.n_q / a.H, rows = a.T * G;
@@ -223,22 +225,17 @@ __global__ void __launch_bounds__(256) kv_attention_kernel(KvAttention a) {
     const uint8_t* vc = a.vc + plane * D;
     const float *ksc = a.ksc + plane, *vsc = a.vsc + plane;
 
-    bf16x8 qf[RT][KS];
-    unsigned long long word[RT];
+    const int row = (rb * WR + wr) * 16 + c;                                 // this lane's column
+    const int t_q = min(row, rows - 1) / G, h_q = hk * G + min(row, rows - 1) % G;
+    bf16x8 qf[KS];
+    const bf16* q = a.q + b * a.qs[0] + t_q * a.qs[1] + h_q * a.qs[2] + 16 * j;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int row = min(rb * (16 * RT) + rt * 16 + c, rows - 1), t = row / G, h = hk * G + row % G;
-        const bf16* q = a.q + b * a.qs[0] + t * a.qs[1] + h * a.qs[2] + 16 * j;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) qf[rt][s] = *(const bf16x8*)(q + 64 * (s >> 1) + 8 * (s & 1));
-        word[rt] = a.tree ? a.tree[(size_t)b * a.T + t] : (2ull << t) - 1;
-    }
-    f32x4 o[RT][DT] = {};
-    float m[RT], l[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) { m[rt] = -INFINITY; l[rt] = 0.f; }
+    for (int s = 0; s < KS; ++s) qf[s] = *(const bf16x8*)(q + 64 * (s >> 1) + 8 * (s & 1));
+    const unsigned long long word = a.tree ? a.tree[(size_t)b * a.T + t_q] : (2ull << t_q) - 1;
+    f32x4 o[DT] = {};
+    float m = -INFINITY, l = 0.f;
 
-    for (int blk = lo + w; blk < hi; blk += 4) {
+    for (int blk = lo + wk; blk < hi; blk += WK) {
         const int t0 = blk * 64;
         u32x4 kf[4][D / 64], vf[DT];
         f32x4 ks[4], vs[4];
@@ -248,164 +245,176 @@ __global__ void __launch_bounds__(256) kv_attention_kernel(KvAttention a) {
             for (int s = 0; s < D / 64; ++s)
                 kf[h][s] = *(const u32x4*)(kc + (size_t)(t0 + 16 * (c >> 2) + 4 * h + (c & 3)) * D + 64 * s + 16 * j);
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            ks[h] = *(const f32x4*)(ksc + t0 + 16 * j + 4 * h);
-            vs[h] = *(const f32x4*)(vsc + t0 + 16 * j + 4 * h);
-        }
+        for (int h = 0; h < 4; ++h) ks[h] = *(const f32x4*)(ksc + t0 + 16 * j + 4 * h);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) vf[dt] = *(const u32x4*)(vc + (size_t)t0 * D + (size_t)(dt * 16 + c) * 64 + 16 * j);
-        const bool edge = t0 + 64 > start;
-        f32x4 s4[RT][4] = {};
+#pragma unroll
+        for (int h = 0; h < 4; ++h) vs[h] = *(const f32x4*)(vsc + t0 + 16 * j + 4 * h);
+        __builtin_amdgcn_sched_barrier(0);      // all of the block's loads are under way before the first is waited for
+        f32x4 s4[4] = {};
 #pragma unroll
         for (int h = 0; h < 4; ++h)
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const bf16x8 f = codes8(kf[h][s >> 1][2 * (s & 1)], kf[h][s >> 1][2 * (s & 1) + 1]);
+            for (int s = 0; s < KS; ++s)
+                s4[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes8(kf[h][s >> 1][2 * (s & 1)], kf[h][s >> 1][2 * (s & 1) + 1]), qf[s], s4[h], 0, 0, 0);
+        uint32_t seen = 0xffffu;                  // bit 4 h + i: this lane's token is visible to its column
+        if (t0 + 64 > start) {
+            seen = 0;
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) s4[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, qf[rt][s], s4[rt][h], 0, 0, 0);
+            for (int i = 0; i < 16; ++i) {
+                const int t = t0 + 16 * j + i, d = t - start;
+                const bool v = t < n && (d < 0 || ((word >> (d & 63)) & 1));
+                seen |= (uint32_t)v << i;
             }
-        bf16x8 ph[RT][2], pl[RT][2];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            uint32_t seen = 0xffffu;              // bit 4 h + i: this lane's token is visible to its column
-            if (edge) {
-                seen = 0;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int t = t0 + 16 * j + i, d = t - start;
-                    const bool v = t < n && (d < 0 || ((word[rt] >> (d & 63)) & 1));
-                    seen |= (uint32_t)v << i;
-                }
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (int h = 0; h < 4; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float s = s4[rt][h][i] * (ks[h][i] * a.scale_log2);
-                    s4[rt][h][i] = (seen >> (4 * h + i)) & 1 ? s : -INFINITY;
-                    top = fmaxf(top, s4[rt][h][i]);
-                }
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float m_new = fmaxf(m[rt], top);
-            const float m_use = m_new == -INFINITY ? 0.f : m_new;
-            if (__any(m_new > m[rt])) {
-                const float alpha = __builtin_amdgcn_exp2f(m[rt] - m_use);       // 0 from -inf
-                l[rt] *= alpha;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[rt][dt][i] *= alpha;
-                m[rt] = m_new;
-            }
-#pragma unroll
-            for (int h = 0; h < 4; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(s4[rt][h][i] - m_use);
-                    l[rt] += p;
-                    const float pv = (seen >> (4 * h + i)) & 1 ? p * vs[h][i] : 0.f;
-                    const bf16 top8 = (bf16)pv;
-                    ph[rt][h >> 1][4 * (h & 1) + i] = top8;
-                    pl[rt][h >> 1][4 * (h & 1) + i] = (bf16)(pv - (float)top8);
-                }
         }
+        float top = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float s = s4[h][i] * (ks[h][i] * a.scale_log2);
+                s4[h][i] = (seen >> (4 * h + i)) & 1 ? s : -INFINITY;
+                top = fmaxf(top, s4[h][i]);
+            }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float m_new = fmaxf(m, top);
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        if (__any(m_new > m)) {
+            const float alpha = __builtin_amdgcn_exp2f(m - m_use);       // 0 from -inf
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[dt][i] *= alpha;
+            m = m_new;
+        }
+        bf16x8 ph[2], pl[2];
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = __builtin_amdgcn_exp2f(s4[h][i] - m_use);
+                l += p;
+                const float pv = (seen >> (4 * h + i)) & 1 ? p * vs[h][i] : 0.f;
+                const bf16 top8 = (bf16)pv;
+                ph[h >> 1][4 * (h & 1) + i] = top8;
+                pl[h >> 1][4 * (h & 1) + i] = (bf16)(pv - (float)top8);
+            }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 const bf16x8 f = codes8(vf[dt][2 * s], vf[dt][2 * s + 1]);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, ph[rt][s], o[rt][dt], 0, 0, 0);
-                    o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, pl[rt][s], o[rt][dt], 0, 0, 0);
-                }
+                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, ph[s], o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, pl[s], o[dt], 0, 0, 0);
             }
     }
 
-    // ---- join the four waves, 16 rows at a time; lane (j, c) of wave w finishes channels 16 dt + 4 j + i, dt = w, w + 4, of row c
+    // ---- join the waves of a row tile; lane (j, c) finishes channels 16 dt + 4 j + i of row c, wave wk those of dt = wk, wk + WK, ...
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    float f[WK];
+    if (WK > 1) {
+        if (j == 0) { lds_m[w][c] = m; lds_l[w][c] = l; }
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        float ls = l[rt];
-        ls += __shfl_xor(ls, 16, 64);
-        ls += __shfl_xor(ls, 32, 64);
-        if (j == 0) { lds_m[w][c] = m[rt]; lds_l[w][c] = ls; }
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) *(f32x4*)lds_o[w][dt][lane] = o[rt][dt];
+        for (int dt = 0; dt < DT; ++dt) *(f32x4*)lds_o[w][dt][lane] = o[dt];
         __syncthreads();
-        float mx = -INFINITY, sum = 0.f, f[4];
+        m = -INFINITY;
+        l = 0.f;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) mx = fmaxf(mx, lds_m[v][c]);
+        for (int v = 0; v < WK; ++v) m = fmaxf(m, lds_m[v * WR + wr][c]);
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            f[v] = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lds_m[v][c] - mx);
-            sum += lds_l[v][c] * f[v];
+        for (int v = 0; v < WK; ++v) {
+            f[v] = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lds_m[v * WR + wr][c] - m);
+            l += lds_l[v * WR + wr][c] * f[v];
         }
-        const int row = rb * (16 * RT) + rt * 16 + c;
-        if (row < rows) {
-            const int t = row / G, h = hk * G + row % G;
-            const size_t orow = ((size_t)b * a.T + t) * a.n_q + h;
-            for (int dt = w; dt < DT; dt += 4) {
-                f32x4 y = {};
+    }
+    if (row >= rows) return;
+    const size_t orow = ((size_t)b * a.T + t_q) * a.n_q + h_q;
 #pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    const f32x4 x = *(const f32x4*)lds_o[v][dt][lane];
+    for (int dd = 0; dd < DT / WK; ++dd) {
+        const int dt = dd * WK + (WK > 1 ? wk : 0);
+        f32x4 y = {};
+        if (WK > 1) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] = __builtin_fmaf(x[i], f[v], y[i]);
-                }
-                if (a.splits == 1) {
-                    bf16x4 z;
+            for (int v = 0; v < WK; ++v) {
+                const f32x4 x = *(const f32x4*)lds_o[v * WR + wr][dt][lane];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) z[i] = sum == 0.f ? (bf16)0.f : (bf16)(y[i] / sum);
-                    *(bf16x4*)(a.out + orow * D + dt * 16 + 4 * j) = z;
-                } else {
-                    *(f32x4*)(a.part_o + (orow * a.splits + split) * D + dt * 16 + 4 * j) = y;
-                }
+                for (int i = 0; i < 4; ++i) y[i] = __builtin_fmaf(x[i], f[v], y[i]);
             }
-            if (a.splits > 1 && w == 0 && j == 0) {
-                a.part_ml[(orow * a.splits + split) * 2] = mx;
-                a.part_ml[(orow * a.splits + split) * 2 + 1] = sum;
-            }
+        } else {
+            y = o[dd];
         }
-        __syncthreads();
+        if (a.splits == 1) {
+            bf16x4 z;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[i] = l == 0.f ? (bf16)0.f : (bf16)(y[i] / l);
+            *(bf16x4*)(a.out + orow * D + dt * 16 + 4 * j) = z;
+        } else {
+            *(f32x4*)(a.part_o + (orow * a.splits + split) * D + dt * 16 + 4 * j) = y;
+        }
+    }
+    if (a.splits > 1 && wk == 0 && j == 0) {
+        a.part_ml[(orow * a.splits + split) * 2] = m;
+        a.part_ml[(orow * a.splits + split) * 2 + 1] = l;
     }
 }
 
-// joins the splits of one output row, in order
+// joins the splits of one output row: 256 / (D / 4) of them at a time, four channels a lane, and these sums in order
 template <int D>
-__global__ void __launch_bounds__(64) kv_attention_join_kernel(const float* part_o, const float* part_ml, bf16* out, int splits) {
+__global__ void __launch_bounds__(256) kv_attention_join_kernel(const float* part_o, const float* part_ml, bf16* out, int splits) {
+    constexpr int LPR = D / 4, P = 256 / LPR;
+    __shared__ f32x4 lds_y[P][LPR];
+    __shared__ float lds_s[P];
     const size_t row = blockIdx.x;
-    const int lane = lane_id();
+    const int tid = (int)threadIdx.x, p = tid / LPR, l = tid % LPR;
     const float* ml = part_ml + row * splits * 2;
     float mx = -INFINITY;
-    for (int s = lane; s < splits; s += 64) mx = fmaxf(mx, ml[2 * s]);
+    for (int s = tid & 63; s < splits; s += 64) mx = fmaxf(mx, ml[2 * s]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-    float sum = 0.f, y[D / 64] = {};
-    for (int s = 0; s < splits; ++s) {
+    f32x4 y = {};
+    float sum = 0.f;
+#pragma unroll 4
+    for (int s = p; s < splits; s += P) {
         const float f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[2 * s] - mx);
-        sum += ml[2 * s + 1] * f;
-        const float* x = part_o + (row * splits + s) * D + lane * (D / 64);
+        const f32x4 x = *(const f32x4*)(part_o + (row * splits + s) * D + 4 * l);
+        sum = __builtin_fmaf(ml[2 * s + 1], f, sum);
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) y[i] = __builtin_fmaf(x[i], f, y[i]);
+        for (int i = 0; i < 4; ++i) y[i] = __builtin_fmaf(x[i], f, y[i]);
     }
+    // a split that saw nothing has m = -inf and weight 0 -- or, where every score is NaN, sums of NaN: they stay
+    lds_y[p][l] = y;
+    if (l == 0) lds_s[p] = sum;
+    __syncthreads();
+    if (p != 0) return;
+    for (int v = 1; v < P; ++v) {
+        sum += lds_s[v];
+        y += lds_y[v][l];
+    }
+    bf16x4 z;
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) out[row * D + lane * (D / 64) + i] = sum == 0.f ? (bf16)0.f : (bf16)(y[i] / sum);
+    for (int i = 0; i < 4; ++i) z[i] = sum == 0.f ? (bf16)0.f : (bf16)(y[i] / sum);
+    *(bf16x4*)(out + row * D + 4 * l) = z;
 }
 
-// How the cache's axis is cut: enough work-groups for the 256 CUs, at least 256 rows (four waves of one block) each.
-static int kv_row_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
-static int kv_splits(int B, int H, int T, int n_q, int cap) {
-    const int rows = T * (n_q / H), rt = kv_row_tiles(rows), rb = (rows + 16 * rt - 1) / (16 * rt);
-    const long long wgs = (long long)B * H * rb;
-    long long s = wgs >= 1024 ? 1 : (1024 + wgs - 1) / wgs;
+// How the work is cut: row tiles and shares of the cache a work-group takes, row blocks, splits of the cache's axis.
+struct KvPlan { int wr, rb, splits; };
+static KvPlan kv_plan(int B, int H, int T, int n_q, int cap) {
+    KvPlan p;
+    const int rows = T * (n_q / H);
+    p.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    p.rb = (rows + 16 * p.wr - 1) / (16 * p.wr);
+    const long long wgs = (long long)B * H * p.rb;
+    const long long s = wgs >= 512 ? 1 : (512 + wgs - 1) / wgs;
     const int most = (cap + 255) / 256;
-    return (int)(s < most ? s : most);
+    p.splits = (int)(s < most ? s : most);
+    return p;
 }
 size_t kv_attention_workspace_bytes(int B, int H, int T, int n_q, int D, int cap) {
     if (B < 1 || H < 1 || T < 1 || n_q < H || D < 1 || cap < 64) return 0;
-    const int s = kv_splits(B, H, T, n_q, cap);
+    const int s = kv_plan(B, H, T, n_q, cap).splits;
     return s == 1 ? 0 : (size_t)B * T * n_q * s * (D + 2) * sizeof(float);
 }
 
@@ -419,23 +428,23 @@ int launch_kv_attention(const KvAttention& in, void* workspace, size_t workspace
     const uintptr_t mis = (uintptr_t)a.kc | (uintptr_t)a.vc | (uintptr_t)a.ksc | (uintptr_t)a.vsc | (uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)workspace;
     PE_REQUIRE((mis & 15) == 0 && ((uintptr_t)a.tree & 7) == 0, "kv_attention: pointers must be 16-byte aligned");
     PE_REQUIRE(a.qs[0] % 8 == 0 && a.qs[1] % 8 == 0 && a.qs[2] % 8 == 0, "kv_attention: strides must be multiples of 8 elements");
-    const int rows = a.T * (a.n_q / a.H), rt = kv_row_tiles(rows), rb = (rows + 16 * rt - 1) / (16 * rt);
-    PE_REQUIRE((long long)a.H * rb <= 65535, "kv_attention: too many heads");
-    a.splits = kv_splits(a.B, a.H, a.T, a.n_q, a.cap);
+    const KvPlan plan = kv_plan(a.B, a.H, a.T, a.n_q, a.cap);
+    PE_REQUIRE((long long)a.H * plan.rb <= 65535, "kv_attention: too many heads");
+    a.splits = plan.splits;
     const size_t need = kv_attention_workspace_bytes(a.B, a.H, a.T, a.n_q, a.D, a.cap);
     PE_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "kv_attention: workspace of %zu bytes, 16-byte aligned, needed", need);
     const size_t out_rows = (size_t)a.B * a.T * a.n_q;
     a.part_o = (float*)workspace;
     a.part_ml = a.part_o ? a.part_o + out_rows * a.splits * a.D : nullptr;
-    const dim3 grid(a.splits, a.H * rb, a.B);
-#define PE_KV_ATT(D, RT) hipLaunchKernelGGL((kv_attention_kernel<D, RT>), grid, dim3(256), 0, stream, a)
-    if (a.D == 64) { if (rt == 1) PE_KV_ATT(64, 1); else if (rt == 2) PE_KV_ATT(64, 2); else PE_KV_ATT(64, 4); }
-    else { if (rt == 1) PE_KV_ATT(128, 1); else if (rt == 2) PE_KV_ATT(128, 2); else PE_KV_ATT(128, 4); }
+    const dim3 grid(a.splits, a.H * plan.rb, a.B);
+#define PE_KV_ATT(D, WR, WK) hipLaunchKernelGGL((kv_attention_kernel<D, WR, WK>), grid, dim3(WR * WK * 64), 0, stream, a)
+    if (a.D == 64) { if (plan.wr == 1) PE_KV_ATT(64, 1, 4); else if (plan.wr == 2) PE_KV_ATT(64, 2, 2); else PE_KV_ATT(64, 4, 1); }
+    else { if (plan.wr == 1) PE_KV_ATT(128, 1, 4); else if (plan.wr == 2) PE_KV_ATT(128, 2, 2); else PE_KV_ATT(128, 4, 1); }
 #undef PE_KV_ATT
     if (const int rc = check_launch("kv_attention_kernel")) return rc;
     if (a.splits > 1) {
-        if (a.D == 64) hipLaunchKernelGGL(kv_attention_join_kernel<64>, dim3((unsigned)out_rows), dim3(64), 0, stream, a.part_o, a.part_ml, a.out, a.splits);
-        else hipLaunchKernelGGL(kv_attention_join_kernel<128>, dim3((unsigned)out_rows), dim3(64), 0, stream, a.part_o, a.part_ml, a.out, a.splits);
+        if (a.D == 64) hipLaunchKernelGGL(kv_attention_join_kernel<64>, dim3((unsigned)out_rows), dim3(256), 0, stream, a.part_o, a.part_ml, a.out, a.splits);
+        else hipLaunchKernelGGL(kv_attention_join_kernel<128>, dim3((unsigned)out_rows), dim3(256), 0, stream, a.part_o, a.part_ml, a.out, a.splits);
         return check_launch("kv_attention_join_kernel");
     }
     return PE_OK;

@@ -4,7 +4,7 @@
 //   r[m] = rsqrt(mean_k x[m,k]^2 + eps) (an RMSNorm whose weight is folded into the weight's columns) or 1
 //   out = y + res,  or with the gated-MLP epilogue  out[m,f] = silu(y[m,f]) * y[m,F+f];  sums in fp32, one rounding to bf16 at the end.
 //
-// Every weight byte is used once, so the kernel is bound by HBM: N K / 2 bytes + N K / g * 2.5.  The products run on
+// Every weight byte is used once, so the kernel is bound by HBM: N K / 2 bytes + 4 N K / g.  The products run on
 // v_mfma_f32_16x16x32_bf16 even for one row: with the weights as the 16-row operand an instruction takes 512 weights in 16 cycles of its
 // SIMD, four times what HBM delivers to a CU, and up to 16 rows of x cost what one does.
 // A code becomes a bf16 by ORing it into the mantissa of 128.0: (u >> 4 i) & 0x000f000f | 0x43004300 is the pair 128 + c, so two weights cost
@@ -16,7 +16,8 @@
 //
 // Layout of the codes: tiles of 16 outputs x 128 inputs, 1 KiB, [N/16][K/128][lane][step]: the lane's four words are its A fragments of the
 // four 32-input steps (output lane & 15, inputs 32 step + 8 (lane >> 4) + e, element e in nibble (e >> 1) + 4 (e & 1)), one coalesced 16-byte load
-// per lane and tile.  Scales and zero points are [N/16][groups][16].  N is padded to 16 with scales of 0, K to 128 (x is read as 0 there).
+// per lane and tile.  Scales and zero points are one word, [N/16][groups][16]: the scale's bf16 and -(128 + zero)
+// as a bf16, exact, above it: each is one instruction away from the fp32 it is used as.  N and K are padded to 16 and 128 with scales of 0.
 //
 // A work-group of W waves takes R tiles of 16 outputs; its waves take turns at the 128-input chunks and join their fp32 sums in LDS in a
 // fixed order: results do not depend on scheduling.  Lanes of rows >= M read row M - 1 again: their columns are never stored.
@@ -28,16 +29,14 @@ namespace pe {
 struct W4Args {
     const bf16* x;
     const u32x4* codes;
-    const bf16* scale;
-    const uint8_t* zero;      // null: 8
+    const u32x4* scale;       // words: scale bf16 | -(128 + zero) bf16 << 16
     const bf16* bias;
     const bf16* res;
     bf16* out;
     long long ldx, ldr, ldo;
     int M, N, K, KC, G;       // KC = chunks of 128 inputs, G = groups (K padded to 128)
     int pair_tiles;           // gated epilogue: tile of the up row = tile of the gate row + pair_tiles
-    float eps;                // >= 0: RMSNorm factor
-    int norm;
+    float eps;
 };
 
 PE_DEV bf16x8 w4_fragment(uint32_t u) {
@@ -47,11 +46,13 @@ PE_DEV bf16x8 w4_fragment(uint32_t u) {
     return __builtin_bit_cast(bf16x8, f);
 }
 
-// MT: tiles of 16 rows of x.  R: weight tiles of a work-group.  GS: 32-input steps of a group (1, 2, 4).
-template <int MT, int R, int W, int GS, bool SWIGLU>
+// MT: tiles of 16 rows of x.  R: weight tiles of a work-group.  W: waves.
+// GS: 32-input steps of a group (1, 2, 4).
+template <int MT, int R, int W, int GS, bool NORM, bool SWIGLU>
 __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
     __shared__ f32x4 part[W][R][64];
     __shared__ float sq[W][MT * 16];
+    constexpr int GC = 4 / GS;                 // groups of a chunk
     const int lane = lane_id(), w = wave_id(), j = lane >> 4, c = lane & 15;
     const int ntiles = (a.N + 15) >> 4;
     int tile[R];
@@ -71,25 +72,31 @@ __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
     for (int e = 0; e < 8; ++e) ones[e] = (bf16)1.0f;
 
     for (int kc = w; kc < a.KC; kc += W) {
-        u32x4 wq[R];
+        u32x4 wq[R], sc[R][GC];
+        bf16x8 b[MT][4];
+        // no branch between the loads; the steps that pad K have scales of 0 (their groups are padding too), their x is any finite part of the row
 #pragma unroll
         for (int r = 0; r < R; ++r) wq[r] = __builtin_nontemporal_load(a.codes + ((size_t)tile[r] * a.KC + kc) * 64 + lane);
-        bf16x8 b[MT][4];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int k = kc * 128 + 32 * s;
+        for (int s = 0; s < 4; ++s)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) b[mt][s] = k < a.K ? *(const bf16x8*)(xrow[mt] + k) : bf16x8{};
-        }
-        if (a.norm) {
+            for (int mt = 0; mt < MT; ++mt) b[mt][s] = *(const bf16x8*)(xrow[mt] + min(kc * 128 + 32 * s, a.K - 32));
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int g = 0; g < GC; ++g) sc[r][g] = a.scale[((size_t)tile[r] * a.G + kc * GC + g) * 4 + j];
+        __builtin_amdgcn_sched_barrier(0);      // or the scheduler sinks the loads to their uses to save registers, one round trip after another
+        if (NORM) {
 #pragma unroll
             for (int s = 0; s < 4; ++s)
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) gram[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[mt][s], b[mt][s], gram[mt], 0, 0, 0);
+                for (int mt = 0; mt < MT; ++mt) {
+                    const bf16x8 f = kc * 128 + 32 * s < a.K ? b[mt][s] : bf16x8{};
+                    gram[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, f, gram[mt], 0, 0, 0);
+                }
         }
 #pragma unroll
-        for (int g = 0; g < 4 / GS; ++g) {
-            const int grp = kc * (4 / GS) + g;
+        for (int g = 0; g < GC; ++g) {
             f32x4 sum[R][MT] = {}, sx[MT] = {};
 #pragma unroll
             for (int s = g * GS; s < (g + 1) * GS; ++s) {
@@ -103,22 +110,18 @@ __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
                 }
             }
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const size_t at = ((size_t)tile[r] * a.G + grp) * 16 + 4 * j;
-                const bf16x4 sc = *(const bf16x4*)(a.scale + at);
-                const uint32_t z = a.zero ? *(const uint32_t*)(a.zero + at) : 0x08080808u;
+            for (int r = 0; r < R; ++r)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float off = -(128.0f + (float)((z >> (8 * i)) & 0xff));
+                    const float scale = __uint_as_float(sc[r][g][i] << 16), off = __uint_as_float(sc[r][g][i] & 0xffff0000u);
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
-                        acc[r][mt][i] = __builtin_fmaf((float)sc[i], __builtin_fmaf(off, sx[mt][i], sum[r][mt][i]), acc[r][mt][i]);
+                        acc[r][mt][i] = __builtin_fmaf(scale, __builtin_fmaf(off, sx[mt][i], sum[r][mt][i]), acc[r][mt][i]);
                 }
-            }
         }
     }
 
-    if (a.norm) {           // the diagonal: row 4 j + i == column c
+    if (NORM) {             // the diagonal: row 4 j + i == column c
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -134,7 +137,7 @@ __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
         for (int o = w; o < OUT; o += W) {
             const int m = mt * 16 + c;
             float rs = 1.0f;
-            if (a.norm) {
+            if (NORM) {
                 float t = 0.f;
 #pragma unroll
                 for (int v = 0; v < W; ++v) t += sq[v][m];
@@ -168,12 +171,14 @@ __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
 }
 
 template <int MT, int R, int W, bool SWIGLU>
-static void w4_launch(const W4Args& a, int gs, hipStream_t stream) {
+static void w4_launch(const W4Args& a, int gs, bool norm, hipStream_t stream) {
     const int tiles = SWIGLU ? a.pair_tiles : (a.N + 15) / 16, per = SWIGLU ? R / 2 : R;
     const dim3 grid((tiles + per - 1) / per), block(W * 64);
-    if (gs == 1) hipLaunchKernelGGL((gemv_w4_kernel<MT, R, W, 1, SWIGLU>), grid, block, 0, stream, a);
-    else if (gs == 2) hipLaunchKernelGGL((gemv_w4_kernel<MT, R, W, 2, SWIGLU>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((gemv_w4_kernel<MT, R, W, 4, SWIGLU>), grid, block, 0, stream, a);
+#define PE_W4(GS, NORM) hipLaunchKernelGGL((gemv_w4_kernel<MT, R, W, GS, NORM, SWIGLU>), grid, block, 0, stream, a)
+    if (gs == 1) { if (norm) PE_W4(1, true); else PE_W4(1, false); }
+    else if (gs == 2) { if (norm) PE_W4(2, true); else PE_W4(2, false); }
+    else { if (norm) PE_W4(4, true); else PE_W4(4, false); }
+#undef PE_W4
 }
 
 int launch_gemv_w4(const W4Problem& p, hipStream_t stream) {
@@ -183,30 +188,34 @@ int launch_gemv_w4(const W4Problem& p, hipStream_t stream) {
     PE_REQUIRE(p.N >= 1 && p.K >= p.group && p.K % p.group == 0, "gemv_w4: N=%d K=%d (K must be a multiple of the group %d)", p.N, p.K, p.group);
     PE_REQUIRE(p.N <= (1 << 26) && p.K <= (1 << 22), "gemv_w4: N=%d K=%d out of range", p.N, p.K);
     PE_REQUIRE(p.ldx >= p.K && p.ldx % 8 == 0 && ((uintptr_t)p.x & 15) == 0, "gemv_w4: rows of x must be 16-byte aligned (ldx=%lld)", p.ldx);
-    PE_REQUIRE(((uintptr_t)p.codes & 15) == 0 && ((uintptr_t)p.scale & 15) == 0 && ((uintptr_t)p.zero & 15) == 0, "gemv_w4: unaligned weight");
+    PE_REQUIRE(((uintptr_t)p.codes & 15) == 0 && ((uintptr_t)p.scale & 15) == 0, "gemv_w4: unaligned weight");
     const int cols = p.swiglu ? p.N / 2 : p.N;
     PE_REQUIRE(!p.swiglu || p.N % 32 == 0, "gemv_w4: the gated epilogue needs a multiple of 16 gate and up rows (N=%d)", p.N);
     PE_REQUIRE(!(p.swiglu && p.res), "gemv_w4: no residual with the gated epilogue");
     PE_REQUIRE(p.ldo >= cols && (!p.res || p.ldr >= cols), "gemv_w4: row stride below the %d columns", cols);
     PE_REQUIRE(!p.norm || p.eps >= 0.f, "gemv_w4: negative eps");
     W4Args a;
-    a.x = (const bf16*)p.x; a.codes = (const u32x4*)p.codes; a.scale = (const bf16*)p.scale; a.zero = (const uint8_t*)p.zero;
+    a.x = (const bf16*)p.x; a.codes = (const u32x4*)p.codes; a.scale = (const u32x4*)p.scale;
     a.bias = (const bf16*)p.bias; a.res = (const bf16*)p.res; a.out = (bf16*)p.out;
     a.ldx = p.ldx; a.ldr = p.ldr; a.ldo = p.ldo;
     a.M = p.M; a.N = p.N; a.K = p.K; a.KC = (p.K + 127) / 128; a.G = a.KC * (128 / p.group);
     a.pair_tiles = p.swiglu ? p.N / 32 : 0;
-    a.norm = p.norm; a.eps = p.eps;
+    a.eps = p.eps;
     const int gs = p.group / 32;
-    const int mt = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
-    if (p.swiglu) {
-        if (mt == 1) w4_launch<1, 2, 4, true>(a, gs, stream);
-        else if (mt == 2) w4_launch<2, 2, 4, true>(a, gs, stream);
-        else w4_launch<4, 2, 4, true>(a, gs, stream);
-    } else {
-        if (mt == 1) w4_launch<1, 1, 8, false>(a, gs, stream);
-        else if (mt == 2) w4_launch<2, 1, 8, false>(a, gs, stream);
-        else w4_launch<4, 1, 8, false>(a, gs, stream);
+    // Weight tiles of a work-group (R): with few tiles every one needs a CU of its own (N = 3584, 224 tiles: R = 1, 16 waves 5.3 us, R = 4 8.2 us); with
+    // many, a work-group's start and end and its reads of x are shared (N = 152064, 9504 tiles: R = 1 80 us, R = 2 69 us, R = 4 54 us).
+    // N = 10000, 625 tiles: 8.8, 8.4, 8.2 us.  From three row tiles on, R = 4 takes the registers of two waves: four waves instead of eight.
+    const int tiles = (p.N + 15) / 16, mt = (p.M + 15) / 16;
+    const int r = tiles <= 256 && !p.swiglu ? 1 : tiles <= (mt >= 3 ? 512 : 1024) ? 2 : 4;
+#define PE_W4_ROWS(MT, W1, W4)                                                                                                   \
+    if (mt == MT) {                                                                                                              \
+        if (p.swiglu) { if (r == 2) w4_launch<MT, 2, 8, true>(a, gs, p.norm, stream); else w4_launch<MT, 4, W4, true>(a, gs, p.norm, stream); } \
+        else if (r == 1) w4_launch<MT, 1, W1, false>(a, gs, p.norm, stream);                                                      \
+        else if (r == 2) w4_launch<MT, 2, 8, false>(a, gs, p.norm, stream);                                                       \
+        else w4_launch<MT, 4, W4, false>(a, gs, p.norm, stream);                                                                  \
     }
+    PE_W4_ROWS(1, 16, 8) else PE_W4_ROWS(2, 8, 8) else PE_W4_ROWS(3, 8, 4) else PE_W4_ROWS(4, 8, 4)
+#undef PE_W4_ROWS
     return check_launch("gemv_w4_kernel");
 }
 

@@ -6,6 +6,7 @@ host.  These are what the `-m gpu` parity tests call, and what `physicedit_amd.d
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -500,51 +501,55 @@ def sdpa_heads64(q: torch.Tensor, kv: torch.Tensor, heads: int) -> torch.Tensor:
 
 
 # ---- the low-bit decode step: 4-bit linears, the e4m3 key/value cache, next-token scores (include/physicedit_amd.h) -----------------
-def _here(*named: Tuple[Optional[torch.Tensor], str]) -> torch.device:
-    """the one device of the given tensors, which has to be the current one: the launch goes to the current stream"""
-    dev = named[0][0].device
-    for t, name in named:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"{name}: expected a CUDA/HIP tensor (physicedit_amd has no CPU path)")
-        if t.device != dev or t.device.index != torch.cuda.current_device():
-            raise ValueError(f"{name}: on {t.device}, but the current device is cuda:{torch.cuda.current_device()} (torch.cuda.device(...))")
-    return dev
+# These are called once per token and layer by programs that do not capture the step, so the checks read each tensor attribute once (an attribute
+# costs about as much as passing an argument) and the launch asks for the raw stream of the current device.
+_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-def _want(t: torch.Tensor, name: str, dtype: torch.dtype, shape: Tuple[int, ...]) -> torch.Tensor:
-    """a contiguous tensor of exactly this type and shape"""
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    return t
+def _stream_of(dev: int, name: str) -> int:
+    """the current stream of device `dev`, which has to be the current device"""
+    if dev < 0:
+        raise ValueError(f"{name}: expected a CUDA/HIP tensor (physicedit_amd has no CPU path)")
+    if dev != _device():
+        raise ValueError(f"{name}: on cuda:{dev}, but the current device is cuda:{_device()} (torch.cuda.device(...))")
+    return _raw_stream(dev)
+
+
+def _at(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, shape, dev: int) -> Optional[int]:
+    """address of a contiguous tensor of exactly this type and shape on device `dev`; None for None"""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
 class W4Weight:
     """A linear's weight [N, K] as 4-bit codes with a scale (and a zero point) per output and `group` inputs, in the layout of pe_gemv_w4
     (include/physicedit_amd.h, pe_w4_weight).  Made by pack_w4 / quantize_w4."""
 
-    def __init__(self, codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor], N: int, K: int, group: int):
-        self.codes, self.scale, self.zero, self.N, self.K, self.group = codes, scale, zero, N, K, group
-        self._c = _lib.W4Weight(codes.data_ptr(), scale.data_ptr(), _ptr(zero), N, K, group)
+    def __init__(self, codes: torch.Tensor, scale: torch.Tensor, N: int, K: int, group: int):
+        self.codes, self.scale, self.N, self.K, self.group = codes, scale, N, K, group
+        self._c = _lib.W4Weight(codes.data_ptr(), scale.data_ptr(), N, K, group)
+        self._ref, self._dev = C.byref(self._c), codes.get_device()
 
     @property
     def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.codes, self.scale, self.zero) if t is not None)
+        return sum(t.numel() * t.element_size() for t in (self.codes, self.scale))
 
 
 def pack_w4(codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor] = None, group: int = 128) -> W4Weight:
     """codes uint8 [N, K/2] (input 2i in the low nibble of byte i), scale bf16 [N, K/group], zero uint8 [N, K/group] in 0 ... 15 or None (8):
     weight = scale * (code - zero).  Lays them out once for gemv_w4."""
-    dev = _here((codes, "codes"), (scale, "scale"), (zero, "zero"))
+    dev = codes.device
+    _stream_of(codes.get_device(), "codes")
     if codes.dim() != 2 or group not in (32, 64, 128):
         raise ValueError(f"pack_w4: codes [N, K/2] and a group of 32, 64 or 128, got {tuple(codes.shape)} and {group}")
     N, K = codes.shape[0], codes.shape[1] * 2
     if N < 1 or K < group or K % group:
         raise ValueError(f"pack_w4: K={K} must be a multiple of the group {group}")
-    _want(codes, "codes", torch.uint8, (N, K // 2)), _want(scale, "scale", BF, (N, K // group))
-    if zero is not None:
-        _want(zero, "zero", torch.uint8, (N, K // group))
+    _at(codes, "codes", torch.uint8, (N, K // 2), dev.index), _at(scale, "scale", BF, (N, K // group), dev.index)
+    _at(zero, "zero", torch.uint8, (N, K // group), dev.index)
     tiles, chunks = (N + 15) // 16, (K + 127) // 128
     full = torch.zeros((tiles * 16, chunks * 64), dtype=torch.uint8, device=dev)
     full[:N, :K // 2] = codes
@@ -555,20 +560,20 @@ def pack_w4(codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tenso
     words[..., 0], words[..., 1] = low[..., 0] | (low[..., 1] << 4), low[..., 2] | (low[..., 3] << 4)
     words[..., 2], words[..., 3] = high[..., 0] | (high[..., 1] << 4), high[..., 2] | (high[..., 3] << 4)
 
-    def per_group(t, fill):
-        padded = torch.full((tiles * 16, chunks * (128 // group)), fill, dtype=t.dtype, device=dev)
-        padded[:N, :K // group] = t
-        return padded.view(tiles, 16, -1).transpose(1, 2).contiguous()
-
-    return W4Weight(words.view(tiles, chunks, 64, 16), per_group(scale, 0), None if zero is None else per_group(zero & 15, 8), N, K, group)
+    pair = torch.zeros((tiles * 16, chunks * (128 // group), 2), dtype=BF, device=dev)      # scale, -(128 + zero)
+    pair[:N, :K // group, 0] = scale
+    pair[:N, :K // group, 1] = -136.0 if zero is None else -128.0 - (zero & 15).to(BF)
+    pair = pair.view(tiles, 16, -1, 2).transpose(1, 2).contiguous()
+    return W4Weight(words.view(tiles, chunks, 64, 16), pair, N, K, group)
 
 
 def quantize_w4(w: torch.Tensor, group: int = 128, zero_point: bool = True, norm_w: Optional[torch.Tensor] = None) -> W4Weight:
     """Round-to-nearest 4-bit form of a bf16 weight [N, K]: per output and group, zero_point: scale = (max(w, 0) - min(w, 0)) / 15 and
     zero = round(-min / scale), else scale = max|w| / 7 and zero = 8.  norm_w [K]: the weight of an RMSNorm in front of the linear, folded
     into the columns first (gemv_w4(norm_eps=...) applies the rest of the norm)."""
-    _chk(w, "w"), _here((w, "w"), (norm_w, "norm_w"))
+    _chk(w, "w"), _stream_of(w.get_device(), "w")
     N, K = w.shape
+    _at(norm_w, "norm_w", BF, (K,), w.get_device())
     if group not in (32, 64, 128) or K % group or K < group:
         raise ValueError(f"quantize_w4: K={K} must be a multiple of the group {group} (32, 64 or 128)")
     codes, scale = torch.empty((N, K // 2), dtype=torch.uint8, device=w.device), torch.empty((N, K // group), dtype=BF, device=w.device)
@@ -596,26 +601,30 @@ def gemv_w4(x: torch.Tensor, w: W4Weight, bias: Optional[torch.Tensor] = None, r
             norm_eps: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [M, K] or [K] (M <= 64 rows; a row stride is fine) @ w.T + bias + res -> [M, N] or [N], one rounding.  epilogue="swiglu": w holds the gate
     rows, then as many up rows (a multiple of 16): silu(gate) * up.  norm_eps: x is RMS-normalised (its norm weight folded into w)."""
-    if epilogue not in ("bias", "swiglu"):
-        raise ValueError(f"gemv_w4: epilogue {epilogue!r} ('bias' or 'swiglu')")
-    if norm_eps is not None and not norm_eps >= 0:
-        raise ValueError(f"gemv_w4: norm_eps={norm_eps}")
-    dev = _here((x, "x"), (w.codes, "w"), (bias, "bias"), (res, "res"), (out, "out"))
-    one = x.dim() == 1
-    rows = x.unsqueeze(0) if one else x
-    if rows.dim() != 2 or rows.dtype != BF or rows.shape[1] != w.K or rows.stride(1) != 1:
-        raise ValueError(f"gemv_w4: expected bf16 rows of {w.K} contiguous values, got {x.dtype} {tuple(x.shape)}")
-    M = rows.shape[0]
     swiglu = epilogue == "swiglu"
-    cols = w.N // 2 if swiglu else w.N
-    shape = (cols,) if one else (M, cols)
-    if bias is not None:
-        _want(bias, "bias", BF, (w.N,))
-    if res is not None:
-        _want(res, "res", BF, shape)
-    out = torch.empty(shape, dtype=BF, device=dev) if out is None else _want(out, "out", BF, shape)
-    check(lib().pe_gemv_w4(rows.data_ptr(), rows.stride(0) if M > 1 else w.K, M, C.byref(w._c), _ptr(bias), _ptr(res), cols, out.data_ptr(), cols,
-                           int(swiglu), -1.0 if norm_eps is None else float(norm_eps), stream_ptr()), "pe_gemv_w4")
+    if not swiglu and epilogue != "bias":
+        raise ValueError(f"gemv_w4: epilogue {epilogue!r} ('bias' or 'swiglu')")
+    if norm_eps is None:
+        norm_eps = -1.0
+    elif not norm_eps >= 0:
+        raise ValueError(f"gemv_w4: norm_eps={norm_eps}")
+    dev, K, cols = w._dev, w.K, w.N // 2 if swiglu else w.N
+    stream = _stream_of(dev, "w")
+    rows, strides = x.shape, x.stride()
+    n = len(rows)
+    if x.dtype is not BF or n not in (1, 2) or rows[-1] != K or strides[-1] != 1 or x.get_device() != dev:
+        raise ValueError(f"gemv_w4: expected bf16 rows of {K} contiguous values on cuda:{dev}, got {x.dtype} {tuple(rows)} on {x.device}")
+    M = 1 if n == 1 else rows[0]
+    shape = (cols,) if n == 1 else (M, cols)
+    if out is None:
+        out = x.new_empty(shape)
+        to = out.data_ptr()
+    else:
+        to = _at(out, "out", BF, shape, dev)
+    rc = lib().pe_gemv_w4(x.data_ptr(), strides[0] if M > 1 else K, M, w._ref, _at(bias, "bias", BF, (w.N,), dev), _at(res, "res", BF, shape, dev), cols,
+                          to, cols, swiglu, norm_eps, stream)
+    if rc:
+        check(rc, "pe_gemv_w4")
     return out
 
 
@@ -633,21 +642,22 @@ class KVCacheE4M3:
         self.k_scale = torch.zeros((batch, n_kv, capacity), dtype=torch.float32, device=device)
         self.v_scale = torch.zeros_like(self.k_scale)
         self._c = _lib.KvCache(self._k.data_ptr(), self._v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), batch, n_kv, capacity, head_dim)
+        self._ref, self._dev = C.byref(self._c), self._k.get_device()
         self.k = self._k.view(F8)
         self.v = self._v.view(F8).transpose(3, 4)
 
-    def start(self, start: torch.Tensor) -> torch.Tensor:
-        return _want(start, "start", torch.int32, (self.batch,))
 
-
-def _rows3(t: torch.Tensor, name: str, batch: int, T: int, heads: int, D: int):
-    """strides (batch, token, head) of a bf16 [batch, T, heads, D] tensor with contiguous channels"""
-    if t.dtype != BF or tuple(t.shape) != (batch, T, heads, D) or t.stride(3) != 1:
-        raise ValueError(f"{name}: expected bf16 [{batch}, {T}, {heads}, {D}] with contiguous channels, got {t.dtype} {tuple(t.shape)}")
-    st = [t.stride(i) if t.shape[i] > 1 else D for i in range(3)]          # the stride of a single entry is never used
-    if any(s % 8 for s in st) or t.data_ptr() % 16:
-        raise ValueError(f"{name}: rows must be 16-byte aligned (strides {tuple(t.stride())})")
-    return (C.c_longlong * 3)(*st)
+def _heads(t: torch.Tensor, name: str, shape, dev: int):
+    """address and strides (batch, token, head) of a bf16 [batch, T, heads, D] tensor with contiguous channels and rows of whole 16 bytes; a
+    dimension of one entry has any stride"""
+    st, at = t.stride(), t.data_ptr()
+    if t.dtype is not BF or t.shape != shape or st[3] != 1 or t.get_device() != dev:
+        raise ValueError(f"{name}: expected bf16 {tuple(shape)} with contiguous channels on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if (st[0] | st[1] | st[2]) & 7:
+        st = tuple(0 if shape[i] == 1 else st[i] for i in range(3))
+    if at & 15 or (st[0] | st[1] | st[2]) & 7:
+        raise ValueError(f"{name}: rows must be 16-byte aligned (strides {t.stride()})")
+    return at, st[:3]
 
 
 def kv_append_e4m3(cache: KVCacheE4M3, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, q: Optional[torch.Tensor] = None,
@@ -656,36 +666,49 @@ def kv_append_e4m3(cache: KVCacheE4M3, k: torch.Tensor, v: torch.Tensor, start: 
     """k, v [batch, T, n_kv, D] (any strides of whole 16 bytes) into rows start[b] ... start[b] + T - 1 (int32 [batch], device) of the cache.  cos, sin
     [rows, D] (bf16 or fp32): k -- and q [batch, T, n_q, D], returned rotated, contiguous -- are rotated with table row positions[b, t] (int32;
     default start[b] + t) first.  Rows past the capacity and sequences with start < 0 are not written (their q comes back zero)."""
-    dev = _here((cache.k_scale, "cache"), (k, "k"), (v, "v"), (start, "start"), (q, "q"), (cos, "cos"), (sin, "sin"), (positions, "positions"), (out, "out"))
+    dev, B, H, D = cache._dev, cache.batch, cache.n_kv, cache.head_dim
+    stream = _stream_of(dev, "cache")
     if k.dim() != 4:
         raise ValueError(f"k: expected [batch, T, n_kv, D], got {tuple(k.shape)}")
-    B, T, H, D = cache.batch, k.shape[1], cache.n_kv, cache.head_dim
-    a = _lib.KvAppendArgs(k=k.data_ptr(), v=v.data_ptr(), k_strides=_rows3(k, "k", B, T, H, D), v_strides=_rows3(v, "v", B, T, H, D), T=T,
-                          start=cache.start(start).data_ptr())
-    if (cos is None) != (sin is None) or (cos is None and (q is not None or positions is not None)):
+    T = k.shape[1]
+    (ka, ks), (va, vs) = _heads(k, "k", (B, T, H, D), dev), _heads(v, "v", (B, T, H, D), dev)
+    qa, qs, qo, n_q, ca, sa, rows, f32 = None, (0, 0, 0), None, 0, None, None, 0, 0
+    if cos is not None and sin is not None:
+        kind, (rows, _) = cos.dtype, cos.shape
+        f32 = kind is torch.float32
+        if not f32 and kind is not BF:
+            raise ValueError(f"cos: expected bf16 or fp32, got {kind}")
+        ca, sa = _at(cos, "cos", kind, (rows, D), dev), _at(sin, "sin", kind, (rows, D), dev)
+    elif cos is not None or sin is not None or q is not None or positions is not None:
         raise ValueError("kv_append_e4m3: q and positions need cos and sin, which come together")
-    if cos is not None:
-        if cos.dim() != 2 or cos.shape[1] != D or cos.dtype not in (BF, torch.float32) or not cos.is_contiguous():
-            raise ValueError(f"cos: expected contiguous bf16 or fp32 [rows, {D}], got {cos.dtype} {tuple(cos.shape)}")
-        _want(sin, "sin", cos.dtype, cos.shape)
-        a.cos, a.sin, a.table_rows, a.table_f32 = cos.data_ptr(), sin.data_ptr(), cos.shape[0], int(cos.dtype == torch.float32)
-        if positions is not None:
-            a.positions = _want(positions, "positions", torch.int32, (B, T)).data_ptr()
     if q is not None:
         if q.dim() != 4:
             raise ValueError(f"q: expected [batch, T, n_q, D], got {tuple(q.shape)}")
-        a.n_q = q.shape[2]
-        a.q, a.q_strides = q.data_ptr(), _rows3(q, "q", B, T, a.n_q, D)
-        out = torch.empty((B, T, a.n_q, D), dtype=BF, device=dev) if out is None else _want(out, "out", BF, (B, T, a.n_q, D))
-        a.q_out = out.data_ptr()
-    check(lib().pe_kv_append_e4m3(C.byref(cache._c), C.byref(a), stream_ptr()), "pe_kv_append_e4m3")
+        n_q = q.shape[2]
+        shape = (B, T, n_q, D)
+        qa, qs = _heads(q, "q", shape, dev)
+        if out is None:
+            out = q.new_empty(shape)
+        qo = _at(out, "out", BF, shape, dev)
+    a = _lib.KvAppendArgs(qa, ka, va, qs, ks, vs, qo, ca, sa, rows, f32, _at(positions, "positions", torch.int32, (B, T), dev),
+                          _at(start, "start", torch.int32, (B,), dev), T, n_q)
+    rc = lib().pe_kv_append_e4m3(cache._ref, C.byref(a), stream)
+    if rc:
+        check(rc, "pe_kv_append_e4m3")
     return out if q is not None else None
+
+
+@functools.lru_cache(maxsize=256)
+def _kv_workspace_bytes(batch: int, n_kv: int, T: int, n_q: int, head_dim: int, capacity: int) -> int:
+    return lib().pe_kv_attention_workspace_bytes(batch, n_kv, T, n_q, head_dim, capacity)
+
+
+_Strides = C.c_longlong * 3
 
 
 def kv_attention_workspace(cache: KVCacheE4M3, T: int, n_q: int) -> torch.Tensor:
     """scratch of kv_attention_e4m3 for calls that want to keep one (one per stream)"""
-    return torch.empty((lib().pe_kv_attention_workspace_bytes(cache.batch, cache.n_kv, T, n_q, cache.head_dim, cache.capacity),),
-                       dtype=torch.uint8, device=cache.k_scale.device)
+    return cache._k.new_empty((_kv_workspace_bytes(cache.batch, cache.n_kv, T, n_q, cache.head_dim, cache.capacity),))
 
 
 def kv_attention_e4m3(q: torch.Tensor, cache: KVCacheE4M3, start: torch.Tensor, tree: Optional[torch.Tensor] = None, scale: Optional[float] = None,
@@ -693,47 +716,51 @@ def kv_attention_e4m3(q: torch.Tensor, cache: KVCacheE4M3, start: torch.Tensor, 
     """Attention of the T <= 64 newest tokens, appended at rows start[b] + t: q [batch, T, n_q, D] -> [batch, T, n_q * D].  Token t sees the cache rows
     below start[b] and new token j where bit j of tree[b, t] (int64) is set; tree None: causal.  scale: default 1 / sqrt(D).  A query that sees
     nothing gives zeros."""
-    dev = _here((cache.k_scale, "cache"), (q, "q"), (start, "start"), (tree, "tree"), (out, "out"), (workspace, "workspace"))
+    dev, B, D = cache._dev, cache.batch, cache.head_dim
+    stream = _stream_of(dev, "cache")
     if q.dim() != 4:
         raise ValueError(f"q: expected [batch, T, n_q, D], got {tuple(q.shape)}")
-    B, T, n_q, D = cache.batch, q.shape[1], q.shape[2], cache.head_dim
-    strides = _rows3(q, "q", B, T, n_q, D)
-    if not 1 <= T <= 64 or n_q % cache.n_kv:
+    _, T, n_q, _ = q.shape
+    qa, qs = _heads(q, "q", (B, T, n_q, D), dev)
+    if not 1 <= T <= 64 or n_q % cache.n_kv or n_q < 1:
         raise ValueError(f"kv_attention_e4m3: {T} new tokens (1 ... 64), {n_q} query heads over {cache.n_kv} kv heads")
-    if tree is not None:
-        _want(tree, "tree", torch.int64, (B, T))
-    out = torch.empty((B, T, n_q * D), dtype=BF, device=dev) if out is None else _want(out, "out", BF, (B, T, n_q * D))
-    ws = kv_attention_workspace(cache, T, n_q) if workspace is None else workspace
-    check(lib().pe_kv_attention_e4m3(C.byref(cache._c), q.data_ptr(), strides, cache.start(start).data_ptr(), _ptr(tree), T, n_q,
-                                     1.0 / math.sqrt(D) if scale is None else float(scale), out.data_ptr(), ws.data_ptr(),
-                                     ws.numel() * ws.element_size(), stream_ptr()), "pe_kv_attention_e4m3")
+    if out is None:
+        out = q.new_empty((B, T, n_q * D))
+        to = out.data_ptr()
+    else:
+        to = _at(out, "out", BF, (B, T, n_q * D), dev)
+    if workspace is None:
+        workspace = kv_attention_workspace(cache, T, n_q)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace: expected a contiguous tensor on cuda:{dev}")
+    rc = lib().pe_kv_attention_e4m3(cache._ref, qa, _Strides(*qs), _at(start, "start", torch.int32, (B,), dev), _at(tree, "tree", torch.int64, (B, T), dev),
+                                    T, n_q, D ** -0.5 if scale is None else scale, to, workspace.data_ptr(), workspace.nbytes, stream)
+    if rc:
+        check(rc, "pe_kv_attention_e4m3")
     return out
 
 
-def _logits_args(logits, counts, penalties, bias, allowed):
-    dev = _here((logits, "logits"), (counts, "counts"), (penalties, "penalties"), (bias, "bias"), (allowed, "allowed"))
-    if logits.dim() != 2 or logits.dtype not in (BF, torch.float32) or logits.stride(1) != 1 or logits.numel() == 0:
-        raise ValueError(f"logits: expected bf16 or fp32 [rows, vocab] with contiguous rows, got {logits.dtype} {tuple(logits.shape)}")
-    R, V = logits.shape
-    a = _lib.LogitsArgs(logits=logits.data_ptr(), ld=logits.stride(0) if R > 1 else V, f32=int(logits.dtype == torch.float32), rows=R, vocab=V)
+def _table(t, name, dtype, R: int, n: int, dev: int):
+    """address and row stride of a table that is there once ([n], stride 0) or for every row ([R, n])"""
+    if t is None:
+        return None, 0
+    return (_at(t, name, dtype, (n,), dev), 0) if t.dim() == 1 else (_at(t, name, dtype, (R, n), dev), n)
 
-    def table(t, name, dtype, n):
-        if t.dim() == 1 and name != "counts":
-            _want(t, name, dtype, (n,))
-            return 0
-        _want(t, name, dtype, (R, n))
-        return n
+
+def _logits_args(logits, counts, penalties, bias, allowed):
+    dev = logits.get_device()
+    stream = _stream_of(dev, "logits")
+    kind, shape, strides = logits.dtype, logits.shape, logits.stride()
+    f32 = kind is torch.float32
+    if not f32 and kind is not BF or len(shape) != 2 or strides[1] != 1 and shape[1] > 1 or 0 in shape:
+        raise ValueError(f"logits: expected bf16 or fp32 [rows, vocab] with contiguous rows, got {kind} {tuple(shape)}")
+    R, V = shape
     if penalties is not None and counts is None:
         raise ValueError("penalties: they need the counts")
-    if counts is not None:
-        a.counts, a.ld_counts = counts.data_ptr(), table(counts, "counts", torch.int16, V)
-    if penalties is not None:
-        a.penalties, a.ld_penalties = penalties.data_ptr(), table(penalties, "penalties", torch.float32, 3)
-    if bias is not None:
-        a.bias, a.ld_bias = bias.data_ptr(), table(bias, "bias", torch.float32, V)
-    if allowed is not None:
-        a.allowed, a.ld_allowed = allowed.data_ptr(), table(allowed, "allowed", torch.int32, (V + 31) // 32)
-    return a, R, V, dev
+    pa, pl = _table(penalties, "penalties", torch.float32, R, 3, dev)
+    ba, bl = _table(bias, "bias", torch.float32, R, V, dev)
+    ma, ml = _table(allowed, "allowed", torch.int32, R, (V + 31) // 32, dev)
+    return _lib.LogitsArgs(logits.data_ptr(), strides[0] if R > 1 else V, f32, R, V, _at(counts, "counts", torch.int16, shape, dev), V, pa, pl, ba, bl, ma, ml), R, V, dev, stream
 
 
 def process_logits(logits: torch.Tensor, counts: Optional[torch.Tensor] = None, penalties: Optional[torch.Tensor] = None,
@@ -742,12 +769,18 @@ def process_logits(logits: torch.Tensor, counts: Optional[torch.Tensor] = None, 
     counts int16 [rows, vocab]: bit 15 (the value is negative) = the prompt holds the token, the rest = how often it was generated (token_counts_add
     keeps them); penalties fp32 [rows, 3] or [3]: repetition (divides positive, multiplies other scores of seen tokens), presence, frequency; bias fp32
     [vocab] or [rows, vocab]; allowed int32 [rows, ceil(vocab / 32)] or [ceil(vocab / 32)]: token v is bit v % 32 of word v / 32, clear = -inf."""
-    a, R, V, dev = _logits_args(logits, counts, penalties, bias, allowed)
-    out = torch.empty((R, V), dtype=torch.float32, device=dev) if out is None else _want(out, "out", torch.float32, (R, V))
-    if out.device != dev:
-        raise ValueError(f"out: on {out.device}, the logits on {dev}")
-    check(lib().pe_process_logits(C.byref(a), out.data_ptr(), stream_ptr()), "pe_process_logits")
+    a, R, V, dev, stream = _logits_args(logits, counts, penalties, bias, allowed)
+    if out is None:
+        out = logits.new_empty((R, V), dtype=torch.float32)
+    rc = lib().pe_process_logits(C.byref(a), _at(out, "out", torch.float32, (R, V), dev), stream)
+    if rc:
+        check(rc, "pe_process_logits")
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _select_workspace_bytes(rows: int, vocab: int) -> int:
+    return lib().pe_select_token_workspace_bytes(rows, vocab)
 
 
 def select_token(logits: torch.Tensor, counts: Optional[torch.Tensor] = None, penalties: Optional[torch.Tensor] = None,
@@ -756,31 +789,37 @@ def select_token(logits: torch.Tensor, counts: Optional[torch.Tensor] = None, pe
                  workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The greedy choice among process_logits' scores, without writing them: int32 [rows], the first maximum (NaN never wins), -1 where everything
     is -inf.  update_counts: counts[row, token] += 1.  step / out_ids (int32, one row): decode_argmax's device-side counter and token list."""
-    a, R, V, dev = _logits_args(logits, counts, penalties, bias, allowed)
+    a, R, V, dev, stream = _logits_args(logits, counts, penalties, bias, allowed)
     if update_counts and counts is None:
         raise ValueError("select_token: update_counts without counts")
-    out = torch.empty((R,), dtype=torch.int32, device=dev) if out is None else _want(out, "out", torch.int32, (R,))
-    if (step is None) != (out_ids is None) or (step is not None and (R != 1 or step.numel() != 1 or out_ids.numel() < 1)):
-        raise ValueError("select_token: step and out_ids come together, for one row")
-    if step is not None:
-        _chk_i32(step, "step"), _chk_i32(out_ids, "out_ids")
+    if out is None:
+        out = logits.new_empty((R,), dtype=torch.int32)
+    ids = at = None
+    room = 0
+    if step is not None or out_ids is not None:
+        if step is None or out_ids is None or R != 1 or step.numel() != 1 or out_ids.dim() != 1 or out_ids.numel() < 1:
+            raise ValueError("select_token: step and out_ids come together, for one row")
+        room = out_ids.numel()
+        ids, at = _at(out_ids, "out_ids", torch.int32, (room,), dev), _at(step, "step", torch.int32, step.shape, dev)
     if workspace is None:
-        workspace = torch.empty((lib().pe_select_token_workspace_bytes(R, V),), dtype=torch.uint8, device=dev)
-    _here((logits, "logits"), (out, "out"), (out_ids, "out_ids"), (step, "step"), (workspace, "workspace"))
-    check(lib().pe_select_token(C.byref(a), out.data_ptr(), int(update_counts), _ptr(out_ids), _ptr(step), 0 if out_ids is None else out_ids.numel(),
-                                workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream_ptr()), "pe_select_token")
+        workspace = logits.new_empty((_select_workspace_bytes(R, V),), dtype=torch.uint8)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace: expected a contiguous tensor on cuda:{dev}")
+    rc = lib().pe_select_token(C.byref(a), _at(out, "out", torch.int32, (R,), dev), update_counts, ids, at, room, workspace.data_ptr(), workspace.nbytes,
+                               stream)
+    if rc:
+        check(rc, "pe_select_token")
     return out
 
 
 def token_counts_add(counts: torch.Tensor, tokens: torch.Tensor, prompt: bool = False) -> torch.Tensor:
     """counts int16 [rows, vocab] of process_logits, in place: every id of tokens int32 [rows, n] counts one more (up to 32767), or with prompt=True
     is marked as part of the prompt.  Ids outside the vocabulary (padding: -1) are skipped."""
-    _here((counts, "counts"), (tokens, "tokens"))
-    if counts.dim() != 2 or counts.dtype != torch.int16 or not counts.is_contiguous() or counts.numel() == 0:
-        raise ValueError(f"counts: expected a contiguous int16 [rows, vocab], got {counts.dtype} {tuple(counts.shape)}")
-    R, V = counts.shape
-    if tokens.dim() != 2 or tokens.shape[1] < 1:
-        raise ValueError(f"tokens: expected int32 [{R}, n], got {tuple(tokens.shape)}")
-    _want(tokens, "tokens", torch.int32, (R, tokens.shape[1]))
-    check(lib().pe_token_counts_add(counts.data_ptr(), V, R, V, tokens.data_ptr(), tokens.shape[1], int(prompt), stream_ptr()), "pe_token_counts_add")
+    dev = counts.get_device()
+    stream = _stream_of(dev, "counts")
+    if counts.dim() != 2 or counts.numel() == 0 or tokens.dim() != 2 or tokens.shape[1] < 1:
+        raise ValueError(f"token_counts_add: counts [rows, vocab] and tokens [rows, n], got {tuple(counts.shape)} and {tuple(tokens.shape)}")
+    (R, V), n = counts.shape, tokens.shape[1]
+    check(lib().pe_token_counts_add(_at(counts, "counts", torch.int16, (R, V), dev), V, R, V, _at(tokens, "tokens", torch.int32, (R, n), dev), n,
+                                    bool(prompt), stream), "pe_token_counts_add")
     return counts
