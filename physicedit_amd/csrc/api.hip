@@ -354,7 +354,7 @@ int pe_kv_append_e4m3(const pe_kv_cache* cache, const pe_kv_append_args* in, voi
     for (int i = 0; i < 3; ++i) { a.qs[i] = in->q_strides[i]; a.ks[i] = in->k_strides[i]; a.vs[i] = in->v_strides[i]; }
     a.q_out = (bf16*)in->q_out; a.cos = in->cos; a.sin = in->sin; a.table_rows = in->table_rows; a.table_f32 = in->table_f32;
     a.positions = in->positions; a.start = in->start; a.T = in->T; a.n_q = in->n_q;
-    a.qk_blocks = a.v_blocks = 0;
+    a.q_groups = a.k_groups = 0;
     return launch_kv_append(a, (hipStream_t)stream);
 }
 

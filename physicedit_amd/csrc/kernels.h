@@ -215,7 +215,7 @@ struct KvAppend {
     int table_rows, table_f32;
     const int *positions, *start;           // [B][T] table rows (null: start + t), [B] cache rows before the new tokens
     int T, n_q;
-    int qk_blocks, v_blocks;                // filled by the launch
+    int q_groups, k_groups;                 // filled by the launch
 };
 int launch_kv_append(const KvAppend& a, hipStream_t stream);
 
@@ -230,7 +230,7 @@ struct KvAttention {
     const unsigned long long* tree;         // [B][T] or null: causal
     int T, n_q;
     float scale_log2;                       // softmax scale * log2(e)
-    int splits;                             // filled by the launch
+    int splits, row_blocks;                 // filled by the launch
     float *part_o, *part_ml;
 };
 size_t kv_attention_workspace_bytes(int B, int H, int T, int n_q, int D, int cap);

@@ -50,7 +50,9 @@ PE_DEV bf16x8 w4_fragment(uint32_t u) {
 // GS: 32-input steps of a group (1, 2, 4).
 template <int MT, int R, int W, int GS, bool NORM, bool SWIGLU>
 __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
-    __shared__ f32x4 part[W][R][64];
+    // a wave's chunk of x, 16 MT rows of 256 bytes, and later its sums
+    constexpr int XB = MT * 4096, PB = R * 1024, SB = XB > PB ? XB : PB;
+    __shared__ __attribute__((aligned(16))) uint8_t stage[W][SB];
     __shared__ float sq[W][MT * 16];
     constexpr int GC = 4 / GS;                 // groups of a chunk
     const int lane = lane_id(), w = wave_id(), j = lane >> 4, c = lane & 15;
@@ -61,10 +63,6 @@ __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
         const int t = SWIGLU ? (int)blockIdx.x * (R / 2) + (r >> 1) : (int)blockIdx.x * R + r;
         tile[r] = SWIGLU ? min(t, a.pair_tiles - 1) + (r & 1) * a.pair_tiles : min(t, ntiles - 1);
     }
-    const bf16* xrow[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) xrow[mt] = a.x + (size_t)min(mt * 16 + c, a.M - 1) * a.ldx + 8 * j;
-
     f32x4 acc[R][MT] = {};
     f32x4 gram[MT] = {};
     bf16x8 ones;
@@ -74,18 +72,28 @@ __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
     for (int kc = w; kc < a.KC; kc += W) {
         u32x4 wq[R], sc[R][GC];
         bf16x8 b[MT][4];
-        // no branch between the loads; the steps that pad K have scales of 0 (their groups are padding too), their x is any finite part of the row
+        // x straight into LDS, four rows of 256 bytes an instruction: 16 consecutive lanes read one row.  (As fragments, 16 lanes read 16 rows and a load
+        // takes 64 steps of the address unit instead of 16: N = 3584, K = 18944, 7 rows 18.6 us against 13.9, 64 rows 74.6 against 38.0.)  Piece p
+        // (16 bytes) of row m goes to slot p ^ (m & 15): the fragment reads below find their 16 rows in 16 different slots.  The steps that pad K have
+        // scales of 0 (their groups are padding too), their x is any part of the row.
+#pragma unroll
+        for (int q = 0; q < MT * 4; ++q)
+            if (4 * q < a.M) {
+                const int m = 4 * q + j, k = kc * 128 + 8 * (c ^ (m & 15));
+                glds16(a.x + (size_t)min(m, a.M - 1) * a.ldx + min(k, a.K - 8), stage[w] + q * 1024);
+            }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int r = 0; r < R; ++r) wq[r] = __builtin_nontemporal_load(a.codes + ((size_t)tile[r] * a.KC + kc) * 64 + lane);
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) b[mt][s] = *(const bf16x8*)(xrow[mt] + min(kc * 128 + 32 * s, a.K - 32));
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int g = 0; g < GC; ++g) sc[r][g] = a.scale[((size_t)tile[r] * a.G + kc * GC + g) * 4 + j];
         __builtin_amdgcn_sched_barrier(0);      // or the scheduler sinks the loads to their uses to save registers, one round trip after another
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) b[mt][s] = *(const bf16x8*)(stage[w] + (mt * 16 + c) * 256 + ((4 * s + j) ^ c) * 16);
         if (NORM) {
 #pragma unroll
             for (int s = 0; s < 4; ++s)
@@ -131,7 +139,7 @@ __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) part[w][r][lane] = acc[r][mt];
+        for (int r = 0; r < R; ++r) *(f32x4*)(stage[w] + (r * 64 + lane) * 16) = acc[r][mt];
         __syncthreads();
         constexpr int OUT = SWIGLU ? R / 2 : R;
         for (int o = w; o < OUT; o += W) {
@@ -147,7 +155,7 @@ __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
 #pragma unroll
             for (int p = 0; p < (SWIGLU ? 2 : 1); ++p) {
 #pragma unroll
-                for (int v = 0; v < W; ++v) y[p] += part[v][SWIGLU ? 2 * o + p : o][lane];
+                for (int v = 0; v < W; ++v) y[p] += *(const f32x4*)(stage[v] + ((SWIGLU ? 2 * o + p : o) * 64 + lane) * 16);
             }
             const int t = (int)blockIdx.x * OUT + o;
             const int n0 = t * 16 + 4 * j, cols = SWIGLU ? a.N / 2 : a.N;
@@ -202,20 +210,18 @@ int launch_gemv_w4(const W4Problem& p, hipStream_t stream) {
     a.pair_tiles = p.swiglu ? p.N / 32 : 0;
     a.eps = p.eps;
     const int gs = p.group / 32;
-    // Weight tiles of a work-group (R): with few tiles every one needs a CU of its own (N = 3584, 224 tiles: R = 1, 16 waves 5.3 us, R = 4 8.2 us); with
-    // many, a work-group's start and end and its reads of x are shared (N = 152064, 9504 tiles: R = 1 80 us, R = 2 69 us, R = 4 54 us).
-    // N = 10000, 625 tiles: 8.8, 8.4, 8.2 us.  From three row tiles on, R = 4 takes the registers of two waves: four waves instead of eight.
+    // Weight tiles (R) and waves (W) of a work-group.  At most a tile per CU: each gets all the waves that fit (N = 3584, K = 18944, one row: R, W = 1, 16
+    // 12.3 us, 1, 8 17.2, 2, 8 20.7).  Some per CU: R = 1 leaves them balanced (N = 10000, K = 3584: 1, 8 7.0 us, 4, 8 8.8).  Many: a work-group's start,
+    // end and reads of x are shared (N = 152064: 1, 8 79.5 us, 2, 8 65.9, 4, 8 53.2).  From two row tiles on x weighs more (20 rows, N = 5001: 1, 8 11.1 us, 2, 8 10.1;
+    // 33: 19.1 and 13.1), from three on its chunks fill the LDS (60 rows, N = 12001: 2, 8 18.1 us, 2, 4 15.0, 4, 4 17.3; 64 rows, N = 152064: 199, 179, 202).
     const int tiles = (p.N + 15) / 16, mt = (p.M + 15) / 16;
-    const int r = tiles <= 256 && !p.swiglu ? 1 : tiles <= (mt >= 3 ? 512 : 1024) ? 2 : 4;
-#define PE_W4_ROWS(MT, W1, W4)                                                                                                   \
-    if (mt == MT) {                                                                                                              \
-        if (p.swiglu) { if (r == 2) w4_launch<MT, 2, 8, true>(a, gs, p.norm, stream); else w4_launch<MT, 4, W4, true>(a, gs, p.norm, stream); } \
-        else if (r == 1) w4_launch<MT, 1, W1, false>(a, gs, p.norm, stream);                                                      \
-        else if (r == 2) w4_launch<MT, 2, 8, false>(a, gs, p.norm, stream);                                                       \
-        else w4_launch<MT, 4, W4, false>(a, gs, p.norm, stream);                                                                  \
-    }
-    PE_W4_ROWS(1, 16, 8) else PE_W4_ROWS(2, 8, 8) else PE_W4_ROWS(3, 8, 4) else PE_W4_ROWS(4, 8, 4)
-#undef PE_W4_ROWS
+    const int size = tiles <= 256 ? 0 : tiles <= (mt >= 3 ? 512 : 1024) ? 1 : 2;
+#define PE_W4(MT, R, W) { if (p.swiglu) w4_launch<MT, (R == 1 ? 2 : R), (R == 1 ? 8 : W), true>(a, gs, p.norm, stream); else w4_launch<MT, R, W, false>(a, gs, p.norm, stream); }
+    if (mt == 1) { if (size == 0) PE_W4(1, 1, 16) else if (size == 1) PE_W4(1, 1, 8) else PE_W4(1, 4, 8) }
+    else if (mt == 2) { if (size == 0) PE_W4(2, 1, 8) else if (size == 1) PE_W4(2, 2, 8) else PE_W4(2, 4, 8) }
+    else if (mt == 3) { if (size == 0) PE_W4(3, 1, 8) else if (size == 1) PE_W4(3, 2, 8) else PE_W4(3, 2, 4) }
+    else { if (size == 0) PE_W4(4, 1, 8) else if (size == 1) PE_W4(4, 2, 8) else PE_W4(4, 2, 4) }
+#undef PE_W4
     return check_launch("gemv_w4_kernel");
 }
 
