@@ -329,13 +329,27 @@ class GraphDecoder:
     launch latency, no Cache object in the loop.  The prefill stays on transformers; its DynamicCache is copied into static planes
     [layer][kv_head][prompt + max_new_tokens][128] that the q/k/v launch appends to (pe_decode_step_*: everything that changes per
     token is read from device memory).  Same kernels, same order, same roundings as `accelerate_decode`, so the tokens are the ones
-    the patched `generate()` produces.  EOS is tested on the host every `chunk` tokens; the overshoot is discarded."""
+    the patched `generate()` produces.  EOS is tested on the host every `chunk` tokens; the overshoot is discarded.
+
+    Low-bit decode (opt-in; the prefill stays bf16): kv_cache="e4m3" keeps keys and values as e4m3 codes with a scale per token and head
+    (pe_kv_append_e4m3 quantises them as they are written, pe_kv_attention_e4m3 reads them back: half the cache bytes), weights="w4" also runs
+    every linear of the step on 4-bit weights with a scale and zero point per output and `w4_group` inputs (pe_gemv_w4: a quarter of the weight
+    bytes; q / k / v and gate / up are one matrix each, the RMSNorm weights folded into their columns).  The 4-bit copies are made at the first
+    call from the model's weights and again when those move or change (call reset() after changing them through `.data`).
+    Penalties and masks: a repetition_penalty or suppress_tokens of the generation config, or generate(prefix_allowed_tokens_fn=), make the
+    next token the first maximum of the processed scores (pe_select_token) instead of the plain arg-max."""
 
     MAX_CACHE_ROWS = 15360          # rows of the static K / V planes pe_decode_step_attention can walk
 
-    def __init__(self, model, chunk: int = 16):
+    def __init__(self, model, chunk: int = 16, weights: Optional[str] = None, kv_cache: Optional[str] = None, w4_group: int = 128):
         from physicedit_amd import ops
         self.ops, self.model, self.chunk = ops, model, chunk
+        self.weights = weights or os.environ.get("PE_DECODE_WEIGHTS", "bf16")
+        self.kv_cache = kv_cache or os.environ.get("PE_DECODE_KV_CACHE", "bf16")
+        self.w4_group = w4_group
+        if self.weights not in ("bf16", "w4") or self.kv_cache not in ("bf16", "e4m3") or (self.weights == "w4" and self.kv_cache != "e4m3"):
+            raise ValueError(f"GraphDecoder: weights={self.weights!r}, kv_cache={self.kv_cache!r} (bf16 and bf16, bf16 and e4m3, or w4 and e4m3)")
+        self._w4 = None             # (fingerprint, 4-bit copies)
         lm = model.model.language_model
         self.lm = lm
         self.layers = list(lm.layers)
@@ -359,6 +373,11 @@ class GraphDecoder:
         # barrier costs 40 - 67 us on the 8-XCD chip (agent-scope atomics serialise at the memory side), ten times the launch boundary it
         # replaces.  Without its barriers (wrong results) the same kernel runs at 362 tok/s: profiles/r06_prologue_notes.md.)
         self.layer_kernel = os.environ.get("PE_DECODE_LAYER_KERNEL", "0") == "1"
+        if self.layer_kernel and self.kv_cache != "bf16":
+            raise ValueError("GraphDecoder: PE_DECODE_LAYER_KERNEL=1 is the bf16 step's")
+        hidden, ff = self.lm.embed_tokens.weight.shape[1], self.layers[0].mlp.gate_proj.out_features
+        if self.weights == "w4" and (hidden % w4_group or ff % w4_group or ff % 16 or (at.q_proj.out_features % w4_group)):
+            raise ValueError(f"GraphDecoder: hidden {hidden}, MLP {ff} and groups of {w4_group} do not fit weights='w4'")
         self._layer_w = None        # per layer: the C struct of its operands (addresses: rebuilt when the weights' fingerprint changes)
         self.split_attention = os.environ.get("PE_DECODE_SPLIT_ATTENTION", "1") != "0"  # pe_decode_step_attention_split (448 work-groups per launch) instead of the 28-work-group launch; same bits
         self._static = {}           # capacity bucket -> static planes, tables, counters and the captured decode step
@@ -373,15 +392,75 @@ class GraphDecoder:
             at, mlp = ly.self_attn, ly.mlp
             ts += [at.q_proj.weight, at.q_proj.bias, at.k_proj.weight, at.k_proj.bias, at.v_proj.weight, at.v_proj.bias, at.o_proj.weight,
                    mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight, ly.input_layernorm.weight, ly.post_attention_layernorm.weight]
-        return tuple((t.data_ptr(), t.dtype, tuple(t.shape)) if t is not None else None for t in ts)
+        # the 4-bit copies hold the weights' values, not their addresses alone: the version counts changes in place
+        version = (lambda t: t._version if not t.is_inference() else 0) if self.weights == "w4" else (lambda t: 0)
+        return tuple((t.data_ptr(), t.dtype, tuple(t.shape), version(t)) if t is not None else None for t in ts)
 
     def reset(self):
-        """Drop the captured graph and its static planes (28 KiB per cache row) now instead of at the next call.  Nothing has to call this
-        for correctness: generate() notices moved / re-allocated weights by itself (_weights_fingerprint) and captures again."""
+        """Drop the captured graph and its static planes (28 KiB per cache row) and the 4-bit weight copies now instead of at the next call.
+        Nothing has to call this for correctness: generate() notices moved / re-allocated weights by itself (_weights_fingerprint) and captures
+        again -- except for weights="w4" after a change through `.data`, which nothing records."""
         self._static = {}
+        self._w4 = None
+
+    def _packed(self, fp):
+        """the 4-bit copies of the weights that `fp` describes: per layer (qkv, its bias, o, gate_up, down), and the lm_head"""
+        if self._w4 is None or self._w4[0] != fp:
+            self._w4 = None                                # the old copies go before the new ones come
+            q4 = lambda w, norm=None: self.ops.quantize_w4(w.contiguous(), self.w4_group, norm_w=norm)
+            layers = []
+            for ly in self.layers:
+                at, mlp = ly.self_attn, ly.mlp
+                bias = [p.bias for p in (at.q_proj, at.k_proj, at.v_proj)]
+                if any(b is None for b in bias):
+                    bias = [torch.zeros(p.out_features, dtype=p.weight.dtype, device=p.weight.device) if p.bias is None else p.bias
+                            for p in (at.q_proj, at.k_proj, at.v_proj)]
+                layers.append((q4(torch.cat([at.q_proj.weight, at.k_proj.weight, at.v_proj.weight]), ly.input_layernorm.weight), torch.cat(bias),
+                               q4(at.o_proj.weight), q4(torch.cat([mlp.gate_proj.weight, mlp.up_proj.weight]), ly.post_attention_layernorm.weight),
+                               q4(mlp.down_proj.weight)))
+            self._w4 = (fp, layers, q4(self.model.lm_head.weight, self.lm.norm.weight))
+        return self._w4
+
+    def _step_low_bit(self, st):
+        """the step's logits with an e4m3 cache and bf16 or 4-bit weights"""
+        ops = self.ops
+        x = ops.decode_embed(self.lm.embed_tokens.weight, st["token"])
+        nq = self.layers[0].self_attn.q_proj.out_features // 128
+        for l, ly in enumerate(self.layers):
+            at, mlp = ly.self_attn, ly.mlp
+            n1, n2 = ly.input_layernorm, ly.post_attention_layernorm
+            e1, e2 = float(n1.variance_epsilon), float(n2.variance_epsilon)
+            if self.weights == "w4":
+                w_qkv, b_qkv, w_o, w_gu, w_down = st["w4"][1][l]
+                q, k, v = ops.gemv_w4(x, w_qkv, bias=b_qkv, norm_eps=e1).view(1, 1, -1, 128).split([nq, self.hkv, self.hkv], dim=2)
+            else:
+                q, k, v = (ops.gemv_norm(x, n1.weight, e1, p.weight, p.bias).view(1, 1, -1, 128) for p in (at.q_proj, at.k_proj, at.v_proj))
+            cache = st["cache"][l]
+            q = ops.kv_append_e4m3(cache, k, v, st["step"], q=q, cos=st["cos"], sin=st["sin"])
+            a = ops.kv_attention_e4m3(q, cache, st["step"], scale=float(at.scaling)).view(-1)
+            if self.weights == "w4":
+                h1 = ops.gemv_w4(a, w_o, res=x)
+                x = ops.gemv_w4(ops.gemv_w4(h1, w_gu, epilogue="swiglu", norm_eps=e2), w_down, res=h1)
+            else:
+                h1 = ops.gemv(a, at.o_proj.weight, None, res=x)
+                x = ops.gemv(ops.gemv_swiglu_norm(h1, n2.weight, e2, mlp.gate_proj.weight, mlp.up_proj.weight), mlp.down_proj.weight, None, res=h1)
+        norm, head = self.lm.norm, self.model.lm_head
+        if self.weights == "w4":
+            return ops.gemv_w4(x, st["w4"][2], bias=head.bias, norm_eps=float(norm.variance_epsilon))
+        return ops.gemv_norm(x, norm.weight, float(norm.variance_epsilon), head.weight, head.bias)
 
     def _step(self, st):
         """one decode step on the current stream (captured); st: dict of static device tensors"""
+        ops = self.ops
+        logits = self._step_low_bit(st) if self.kv_cache == "e4m3" else self._step_bf16(st)
+        if st["select"]:
+            ops.select_token(logits.view(1, -1), counts=st["counts"], penalties=st["penalties"], allowed=st["allowed"], update_counts=True,
+                             out=st["token"], out_ids=st["out_ids"], step=st["step"])
+        else:
+            ops.decode_argmax(logits, st["token"], st["out_ids"], st["step"])
+
+    def _step_bf16(self, st):
+        """the step's logits with bf16 weights and cache"""
         ops = self.ops
         x = ops.decode_embed(self.lm.embed_tokens.weight, st["token"])
         if self.layer_kernel:
@@ -399,13 +478,25 @@ class GraphDecoder:
             hid = ops.gemv_swiglu_norm(h1, ly.post_attention_layernorm.weight, float(ly.post_attention_layernorm.variance_epsilon),
                                        mlp.gate_proj.weight, mlp.up_proj.weight)
             x = ops.gemv(hid, mlp.down_proj.weight, None, res=h1)
-        logits = ops.gemv_norm(x, self.lm.norm.weight, float(self.lm.norm.variance_epsilon), self.model.lm_head.weight,
-                               self.model.lm_head.bias)
-        ops.decode_argmax(logits, st["token"], st["out_ids"], st["step"])
+        return ops.gemv_norm(x, self.lm.norm.weight, float(self.lm.norm.variance_epsilon), self.model.lm_head.weight,
+                             self.model.lm_head.bias)
+
+    def _allow(self, st, ids):
+        """the mask of allowed tokens: all (None) or the given ids, without the generation config's suppress_tokens"""
+        V = st["counts"].shape[1]
+        bits = torch.full((V + 31,), ids is None, dtype=torch.bool)
+        if ids is not None:
+            bits[torch.as_tensor(ids, dtype=torch.long)] = True
+        if getattr(self.model.generation_config, "suppress_tokens", None):
+            bits[torch.as_tensor(list(self.model.generation_config.suppress_tokens), dtype=torch.long)] = False
+        words = (bits[:V + (-V) % 32].view(-1, 32).long() << torch.arange(32)).sum(1)
+        st["allowed"].copy_(torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32))
 
     @torch.no_grad()
-    def generate(self, max_new_tokens: int = 1000, **model_inputs) -> torch.Tensor:
-        """-> [1, prompt + generated] token ids, like GenerationMixin.generate for a batch of one (EOS included when it came)."""
+    def generate(self, max_new_tokens: int = 1000, prefix_allowed_tokens_fn=None, **model_inputs) -> torch.Tensor:
+        """-> [1, prompt + generated] token ids, like GenerationMixin.generate for a batch of one (EOS included when it came).
+        prefix_allowed_tokens_fn(0, ids so far) -> the token ids allowed next, as in transformers (a grammar's mask): asked before every token, so
+        the step is replayed one token at a time."""
         model, dev = self.model, self.lm.embed_tokens.weight.device
         ids = model_inputs["input_ids"]
         if ids.shape[0] != 1:
@@ -415,6 +506,8 @@ class GraphDecoder:
         eos = gen.eos_token_id
         eos = set() if eos is None else set(eos if isinstance(eos, (list, tuple)) else [eos])
         min_new = int(getattr(gen, "min_new_tokens", 0) or 0)
+        penalty = float(getattr(gen, "repetition_penalty", None) or 1.0)
+        select = prefix_allowed_tokens_fn is not None or penalty != 1.0 or bool(getattr(gen, "suppress_tokens", None))
         cap = Lp + max_new_tokens
         if cap > self.MAX_CACHE_ROWS:
             raise ValueError(f"GraphDecoder.generate: prompt + max_new_tokens exceeds the decode attention's {self.MAX_CACHE_ROWS}-row cache")
@@ -423,7 +516,7 @@ class GraphDecoder:
             out = model(**model_inputs, use_cache=True, logits_to_keep=1)
         except TypeError:
             out = model(**model_inputs, use_cache=True)
-        first = int(out.logits[0, -1].float().argmax())
+        last_logits = out.logits[:, -1].contiguous()
         past = out.past_key_values
         L = len(self.layers)
         # ---- static state, one set per capacity bucket, kept across calls WITH its captured graph: nothing the graph's launches take
@@ -436,12 +529,17 @@ class GraphDecoder:
         if st is not None and st.get("weights") != fp:
             st = None                                      # the weights moved since the capture: those launches point at the old ones
         if st is None:
-            st = {"kc": torch.zeros((L, self.hkv, bucket, 128), dtype=torch.bfloat16, device=dev), "base": 0, "cap": bucket,
+            kc = torch.zeros((L if self.kv_cache == "bf16" else 0, self.hkv, bucket, 128), dtype=torch.bfloat16, device=dev)
+            st = {"kc": kc, "base": 0, "cap": bucket, "select": False,
                   "cos": torch.zeros((bucket, 128), dtype=torch.bfloat16, device=dev),
                   "token": torch.zeros(1, dtype=torch.int32, device=dev), "step": torch.zeros(1, dtype=torch.int32, device=dev),
                   "out_ids": torch.zeros(bucket, dtype=torch.int32, device=dev), "graph": None, "weights": fp}
             st["vc"] = torch.zeros_like(st["kc"])
-            if self.split_attention:     # scratch of the three-launch single-query attention (layers run one after the other: one buffer)
+            if self.kv_cache == "e4m3":
+                st["cache"] = [self.ops.KVCacheE4M3(1, self.hkv, bucket, 128, device=dev) for _ in range(L)]
+            if self.weights == "w4":
+                st["w4"] = self._packed(fp)
+            if self.split_attention and self.kv_cache == "bf16":     # scratch of the three-launch single-query attention (layers run one after the other: one buffer)
                 st["attn_ws"] = self.ops.decode_attention_workspace(len(self.layers[0].self_attn.q_proj.weight) // 128, bucket, dev)
             st["sin"] = torch.zeros_like(st["cos"])
             if self.layer_kernel:
@@ -454,7 +552,16 @@ class GraphDecoder:
                     ly.mlp.down_proj.weight, ly.input_layernorm.weight, ly.input_layernorm.variance_epsilon, ly.post_attention_layernorm.weight,
                     ly.post_attention_layernorm.variance_epsilon) for ly in self.layers]
             self._static = {bucket: st}                    # one bucket alive at a time (28 KiB per row of capacity and plane pair)
+        if select != st["select"]:       # the captured step ends in the other choice of a token
+            st["graph"], st["select"] = None, select
+        if select and "counts" not in st:
+            V = last_logits.shape[1]
+            st["counts"] = torch.zeros((1, V), dtype=torch.int16, device=dev)
+            st["penalties"] = torch.zeros((3,), dtype=torch.float32, device=dev)
+            st["allowed"] = torch.zeros(((V + 31) // 32,), dtype=torch.int32, device=dev)
         kc, vc = st["kc"], st["vc"]
+        if self.kv_cache == "e4m3":
+            nothing = torch.zeros((1,), dtype=torch.int32, device=dev)
         for l in range(L):
             if hasattr(past, "layers"):                    # transformers >= 4.54: DynamicCache.layers[l].keys / .values
                 k, v = past.layers[l].keys, past.layers[l].values
@@ -462,9 +569,22 @@ class GraphDecoder:
                 k, v = past.key_cache[l], past.value_cache[l]
             else:
                 k, v = past[l][0], past[l][1]
+            if self.kv_cache == "e4m3":
+                self.ops.kv_append_e4m3(st["cache"][l], k.transpose(1, 2), v.transpose(1, 2), nothing)
+                continue
             kc[l, :, :Lp].copy_(k[0])
             vc[l, :, :Lp].copy_(v[0])
         del out, past
+        if select:
+            st["counts"].zero_()
+            self.ops.token_counts_add(st["counts"], ids.to(device=dev, dtype=torch.int32).contiguous(), prompt=True)
+            st["penalties"].copy_(torch.tensor([penalty, 0.0, 0.0]))
+            self._allow(st, prefix_allowed_tokens_fn(0, ids[0]) if prefix_allowed_tokens_fn else None)
+            first = int(self.ops.select_token(last_logits, counts=st["counts"], penalties=st["penalties"], allowed=st["allowed"], update_counts=True))
+            if first < 0:
+                raise RuntimeError("GraphDecoder.generate: no token is allowed")
+        else:
+            first = int(last_logits[0].float().argmax())
         # ---- rotary tables of the decode positions: position of generated token t = prompt length + t + rope_delta on all 3 axes
         delta = getattr(model.model, "rope_deltas", None)
         delta = int(delta.reshape(-1)[0]) if delta is not None else 0
@@ -480,6 +600,7 @@ class GraphDecoder:
             side.wait_stream(torch.cuda.current_stream(dev))
             with torch.cuda.stream(side):
                 if st["graph"] is None:
+                    kept = st["counts"].clone() if select else None        # the warm-up's token is not a generated one
                     st["step"].fill_(Lp)
                     st["token"].fill_(first)
                     self._step(st)                         # warm-up outside the capture (lazy module loads, allocator)
@@ -489,12 +610,16 @@ class GraphDecoder:
                         self._step(st)
                     st["graph"] = graph
                     self.captures += 1
+                    if select:
+                        st["counts"].copy_(kept)
                 graph = st["graph"]
                 st["step"].fill_(Lp)
                 st["token"].fill_(first)
                 done = 0
                 while done < n_steps:
-                    n = min(self.chunk, n_steps - done)
+                    n = min(self.chunk if prefix_allowed_tokens_fn is None else 1, n_steps - done)
+                    if prefix_allowed_tokens_fn is not None:
+                        self._allow(st, prefix_allowed_tokens_fn(0, torch.cat([ids[0], torch.tensor(tokens, dtype=ids.dtype, device=ids.device)])))
                     for _ in range(n):
                         graph.replay()
                     new = st["out_ids"][Lp + done:Lp + done + n].tolist()            # synchronises
@@ -502,6 +627,8 @@ class GraphDecoder:
                         raise RuntimeError("pe_decode_layer: a grid barrier timed out (the decode grid was not fully resident); "
                                            "set PE_DECODE_LAYER_KERNEL=0")
                     done += n
+                    if select and min(new) < 0:
+                        raise RuntimeError("GraphDecoder.generate: no token is allowed")
                     stop = next((i for i, t in enumerate(new) if t in eos and len(tokens) + i + 1 >= max(min_new, 1)), None)
                     if stop is not None:
                         tokens += new[:stop + 1]
@@ -589,7 +716,9 @@ class PromptPrologue:
     (pipe, prompt=, negative_prompt=, edit_image=, cfg=, have_text_reasoning=) -> (posi, nega) dicts."""
 
     def __init__(self, text_encoder, processor, tokenizer=None, device="cuda", torch_dtype=torch.bfloat16, decode_gemv: bool = True,
-                 decode_graph: bool = True):
+                 decode_graph: bool = True, decode_weights: Optional[str] = None, decode_kv_cache: Optional[str] = None):
+        """decode_weights / decode_kv_cache: GraphDecoder's weights ("bf16", "w4") and kv_cache ("bf16", "e4m3"); by default the environment's
+        PE_DECODE_WEIGHTS / PE_DECODE_KV_CACHE, else bf16."""
         self.text_encoder = text_encoder
         self.decode_gemv = 0
         self.graph_decoder = None
@@ -597,8 +726,10 @@ class PromptPrologue:
             self.decode_gemv = accelerate_decode(text_encoder)
             if decode_graph:
                 try:
-                    self.graph_decoder = GraphDecoder(text_encoder)
+                    self.graph_decoder = GraphDecoder(text_encoder, weights=decode_weights, kv_cache=decode_kv_cache)
                 except (ValueError, AttributeError) as e:            # another architecture / dtype: transformers' generate()
+                    if (decode_weights or "bf16", decode_kv_cache or "bf16") != ("bf16", "bf16"):
+                        raise                                          # asked for by name: no silent bf16
                     print(f"[prompt_prologue] captured decode step not available ({e}); using generate()")
         self.processor = processor
         self.tokenizer = tokenizer if tokenizer is not None else processor.tokenizer
@@ -610,6 +741,8 @@ class PromptPrologue:
         self.boi_token_id = tok.convert_tokens_to_ids("<begin_of_img>")
         self.eoi_token_id = tok.convert_tokens_to_ids("<end_of_img>")
         self.last_physical_txt: Optional[str] = None
+        # (batch index, ids so far) -> allowed ids, as transformers' prefix_allowed_tokens_fn: a grammar for physical_text's answer
+        self.allowed_tokens_fn = None
         # (prompt, negative prompt, image bytes, cfg, reasoning) -> results of __call__.  The prologue is deterministic (greedy
         # decoding, no dropout), and its greedy decode can take as long as the whole denoising loop (profiles/r02_prologue.json),
         # so repeated edits of one (image, instruction) pair -- other seeds, step counts, sizes -- skip it.  0 disables.
@@ -641,19 +774,21 @@ class PromptPrologue:
 
     # ---- PhysicalVerbalEmbedder at inference (:943-967, :859-873) -------------------------------------------
     @torch.no_grad()
-    def generate_ids(self, model_inputs, max_new_tokens: int):
+    def generate_ids(self, model_inputs, max_new_tokens: int, prefix_allowed_tokens_fn=None):
         """`text_encoder.generate(**model_inputs, max_new_tokens=...)`: through the captured decode step when the encoder qualifies
-        (bf16 on the GPU, greedy), through transformers otherwise."""
+        (bf16 on the GPU, greedy; a repetition penalty, suppressed tokens and a callback for the allowed ones included), through
+        transformers otherwise."""
         gen = self.text_encoder.generation_config
         plain_greedy = (not getattr(gen, "do_sample", False) and (getattr(gen, "num_beams", 1) or 1) == 1
-                        and (getattr(gen, "repetition_penalty", None) or 1.0) == 1.0
+                        and (getattr(gen, "repetition_penalty", None) or 1.0) > 0.0
                         and not getattr(gen, "no_repeat_ngram_size", 0) and not getattr(gen, "bad_words_ids", None)
-                        and not getattr(gen, "suppress_tokens", None) and not getattr(gen, "forced_eos_token_id", None))
+                        and not getattr(gen, "forced_eos_token_id", None))
         ids = model_inputs["input_ids"]
         if (self.graph_decoder is not None and plain_greedy and ids.shape[0] == 1
                 and ids.shape[1] + max_new_tokens <= GraphDecoder.MAX_CACHE_ROWS):        # longer: the reference's own path
-            return self.graph_decoder.generate(max_new_tokens=max_new_tokens, **model_inputs)
-        return self.text_encoder.generate(**model_inputs, max_new_tokens=max_new_tokens)
+            return self.graph_decoder.generate(max_new_tokens=max_new_tokens, prefix_allowed_tokens_fn=prefix_allowed_tokens_fn, **model_inputs)
+        more = {} if prefix_allowed_tokens_fn is None else {"prefix_allowed_tokens_fn": prefix_allowed_tokens_fn}
+        return self.text_encoder.generate(**model_inputs, max_new_tokens=max_new_tokens, **more)
 
     def physical_text(self, prompt: str, edit_image: Image.Image) -> str:
         messages = [
@@ -663,7 +798,7 @@ class PromptPrologue:
         ]
         text = self.processor.apply_chat_template(messages, tokenize=False, add_generation_prompt=True, add_vision_id=True)
         model_inputs = self.processor(text=[text], images=resize_for_vl(edit_image), padding=True, return_tensors="pt").to(self.device)
-        decoded_ids = self.generate_ids(model_inputs, max_new_tokens=1000)
+        decoded_ids = self.generate_ids(model_inputs, max_new_tokens=1000, prefix_allowed_tokens_fn=self.allowed_tokens_fn)
         trimmed = [out_ids[len(in_ids):] for in_ids, out_ids in zip(model_inputs["input_ids"], decoded_ids)]
         decoded = self.tokenizer.batch_decode(trimmed, skip_special_tokens=True, clean_up_tokenization_spaces=False)[0]
         try:
@@ -722,9 +857,12 @@ class PromptPrologue:
         """`physical_txt`: reasoning text supplied by the caller instead of generated (PhysicalVerbalEmbedder.process, :976-983:
         the annotated-triplet branch, taken when the rules / key frames / input image of a dataset sample are all given)."""
         clone = lambda d: {k: (v.clone() if isinstance(v, torch.Tensor) else v) for k, v in d.items()}   # callers mutate prompt_emb
-        key = (prompt, negative_prompt, self._image_key(edit_image), bool(cfg), bool(have_text_reasoning), physical_txt)
+        gen = getattr(self.text_encoder, "generation_config", None)
+        key = (prompt, negative_prompt, self._image_key(edit_image), bool(cfg), bool(have_text_reasoning), physical_txt,
+               getattr(gen, "repetition_penalty", None), tuple(getattr(gen, "suppress_tokens", None) or ()))
         given = physical_txt
-        if self.cache_size and key in self._cache:
+        cache_size = self.cache_size if self.allowed_tokens_fn is None else 0          # a callback's answers are its own
+        if cache_size and key in self._cache:
             self._cache.move_to_end(key)
             posi, nega, self.last_physical_txt = self._cache[key]
             return clone(posi), clone(nega)
@@ -739,7 +877,7 @@ class PromptPrologue:
         self.last_physical_txt = physical_txt
         posi = self.embed(prompt, edit_image, physical_txt)
         nega = self.embed(negative_prompt, edit_image, None) if cfg else dict(posi)
-        if self.cache_size:
+        if cache_size:
             self._cache[key] = (clone(posi), clone(nega), physical_txt)
             while len(self._cache) > self.cache_size:
                 self._cache.popitem(last=False)

@@ -1,0 +1,251 @@
+"""`-m gpu`: the low-bit operators together, as GraphDecoder's captured decode step runs them: penalties and masks against transformers'
+generate(), the e4m3 cache and 4-bit weights against the same step written out in plain torch."""
+import copy
+
+import pytest
+import torch
+
+from test_gpu_lowbit import attention_reference, quantise, rotate
+
+pytestmark = pytest.mark.gpu
+BF, F64 = torch.bfloat16, torch.float64
+
+
+@pytest.fixture(scope="module")
+def model():
+    """a random Qwen2.5-VL text encoder of the real widths with 3 layers and a small vocabulary"""
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from transformers import Qwen2_5_VLConfig, Qwen2_5_VLForConditionalGeneration
+    from diffsynth.pipelines import prompt_prologue as PP
+    cfg = copy.deepcopy(PP.TEXT_ENCODER_CONFIG)
+    cfg["text_config"].update(num_hidden_layers=3, vocab_size=4001, bos_token_id=1, eos_token_id=2, pad_token_id=0)
+    cfg["vision_config"].update(depth=1, fullatt_block_indexes=[0])
+    cfg.update(image_token_id=10, video_token_id=11, vision_start_token_id=12, vision_end_token_id=13, bos_token_id=1, eos_token_id=2)
+    old = torch.get_default_dtype()
+    torch.set_default_dtype(BF)
+    try:
+        with torch.device("cuda"):
+            m = Qwen2_5_VLForConditionalGeneration(Qwen2_5_VLConfig(**cfg))
+    finally:
+        torch.set_default_dtype(old)
+    g = torch.Generator(device="cuda").manual_seed(11)
+    with torch.no_grad():
+        for name, p in m.named_parameters():
+            if p.dim() >= 2:
+                p.normal_(0.0, 0.03, generator=g)
+            elif "norm" in name:
+                p.normal_(1.0, 0.1, generator=g)
+            else:
+                p.normal_(0.0, 0.02, generator=g)
+    m.eval()
+    m.generation_config.do_sample = False
+    m.generation_config.pad_token_id, m.generation_config.eos_token_id = 0, None
+    assert PP.accelerate_decode(m) > 0
+    return m
+
+
+@pytest.fixture
+def config(model):
+    """the model's generation config, put back afterwards"""
+    old = copy.deepcopy(model.generation_config)
+    yield model.generation_config
+    model.generation_config = old
+
+
+def prompt(n, seed=3):
+    ids = torch.randint(20, 3900, (1, n), generator=torch.Generator().manual_seed(seed)).cuda()
+    return {"input_ids": ids, "attention_mask": torch.ones_like(ids)}
+
+
+def decoder(model, **kw):
+    from diffsynth.pipelines import prompt_prologue as PP
+    return PP.GraphDecoder(model, chunk=8, **kw)
+
+
+def test_penalties_and_masks_match_generate(model, config):
+    """the same kernels decode both ways and both choices are made in fp32 on the same logits: identical tokens"""
+    dec = decoder(model)
+    inputs = prompt(37)
+    plain = dec.generate(max_new_tokens=24, **inputs)
+    config.repetition_penalty = 1.3
+    with torch.no_grad():
+        want = model.generate(**inputs, max_new_tokens=24, min_new_tokens=24)
+    got = dec.generate(max_new_tokens=24, **inputs)
+    assert torch.equal(got, want)
+    config.suppress_tokens = sorted(set(want[0, 37:45].tolist()))                 # what it liked best is taken away
+    with torch.no_grad():
+        want2 = model.generate(**inputs, max_new_tokens=24, min_new_tokens=24)
+    got2 = dec.generate(max_new_tokens=24, **inputs)
+    assert torch.equal(got2, want2) and not set(config.suppress_tokens) & set(got2[0, 37:].tolist())
+    assert dec.captures == 2                                                      # one plain step, one that selects
+    # a grammar: even and odd ids in turn, from a window that moves with the last token
+    def grammar(batch, ids):
+        last = int(ids[-1])
+        return [i for i in range(max(20, last - 900), min(4000, last + 900)) if (i - last) % 2 == 1]
+    config.suppress_tokens = None
+    with torch.no_grad():
+        want3 = model.generate(**inputs, max_new_tokens=12, min_new_tokens=12, prefix_allowed_tokens_fn=grammar)
+    got3 = dec.generate(max_new_tokens=12, prefix_allowed_tokens_fn=grammar, **inputs)
+    assert torch.equal(got3, want3)
+    toks = got3[0, 36:].tolist()
+    assert all((b - a) % 2 for a, b in zip(toks, toks[1:])) and dec.captures == 2
+    with pytest.raises(RuntimeError, match="no token is allowed"):
+        dec.generate(max_new_tokens=4, prefix_allowed_tokens_fn=lambda b, i: [] if i.numel() > 38 else [500], **inputs)
+    config.repetition_penalty = 1.0
+    assert torch.equal(dec.generate(max_new_tokens=24, **inputs), plain)          # and back to the plain arg-max
+
+
+def dequantised(w4):
+    """the weight that a W4Weight stands for, from the layout's definition (include/physicedit_amd.h, pe_w4_weight), exactly"""
+    words = w4.codes.contiguous().view(torch.int32).view(*w4.codes.shape[:2], 4, 16, 4)              # tile, chunk, lane / 16, lane % 16, step
+    codes = torch.stack([(words >> (4 * (e // 2 + 4 * (e % 2)))) & 15 for e in range(8)], -1)
+    codes = codes.permute(0, 3, 1, 4, 2, 5).reshape(words.shape[0] * 16, -1)[:w4.N, :w4.K].to(F64)
+    scale, zero = w4.scale[..., 0].to(F64), -128 - w4.scale[..., 1].to(F64)
+    per_input = lambda t: t.transpose(1, 2).reshape(words.shape[0] * 16, -1).repeat_interleave(w4.group, 1)[:w4.N, :w4.K]
+    return per_input(scale) * (codes - per_input(zero))
+
+
+@torch.no_grad()
+def plain_step(dec, st):
+    """one step of the low-bit decode in plain torch: 64-bit products, each operator's result rounded to bf16 once -> logits, and the caches' new rows"""
+    model, lm, pos = dec.model, dec.lm, int(st["step"])
+    r = lambda t: t.to(BF).to(F64)
+    x = lm.embed_tokens.weight[int(st["token"])].to(F64)
+    rows = []
+    for l, ly in enumerate(dec.layers):
+        at, mlp = ly.self_attn, ly.mlp
+        norm = lambda t, n: t / (t.square().mean() + n.variance_epsilon).sqrt()
+        if dec.weights == "w4":
+            qkv_w, qkv_b, o_w, gu_w, down_w = st["w4"][1][l]
+            qkv = r(dequantised(qkv_w) @ norm(x, ly.input_layernorm) + qkv_b.to(F64))
+        else:
+            n1 = r(r(norm(x, ly.input_layernorm)) * ly.input_layernorm.weight.to(F64))
+            qkv = r(torch.cat([p.weight.to(F64) @ n1 + p.bias.to(F64) for p in (at.q_proj, at.k_proj, at.v_proj)]))
+        q, k, v = qkv.view(-1, 128).split([28, 4, 4])
+        cos, sin = st["cos"][pos].to(F64), st["sin"][pos].to(F64)
+        q = rotate(q, cos, sin).to(BF)
+        rows.append((*quantise(rotate(k, cos, sin).float()), *quantise(v.float())))
+        a = r(attention_reference(q.view(1, 1, 28, 128), st["cache"][l], st["step"], scale=float(at.scaling))[0].view(-1))
+        if dec.weights == "w4":
+            h = r(x + dequantised(o_w) @ a)
+            gate, up = (dequantised(gu_w) @ norm(h, ly.post_attention_layernorm)).chunk(2)
+            x = r(h + dequantised(down_w) @ r(gate * torch.sigmoid(gate) * up))
+        else:
+            h = r(x + r(at.o_proj.weight.to(F64) @ a))
+            n2 = r(r(norm(h, ly.post_attention_layernorm)) * ly.post_attention_layernorm.weight.to(F64))
+            gate, up = r(mlp.gate_proj.weight.to(F64) @ n2), r(mlp.up_proj.weight.to(F64) @ n2)
+            x = r(h + r(mlp.down_proj.weight.to(F64) @ r(r(gate * torch.sigmoid(gate)) * up)))
+    if dec.weights == "w4":
+        return r(dequantised(st["w4"][2]) @ norm(x, lm.norm)), rows
+    return r(model.lm_head.weight.to(F64) @ r(r(norm(x, lm.norm)) * lm.norm.weight.to(F64))), rows
+
+
+@pytest.mark.parametrize("weights", ["bf16", "w4"])
+def test_low_bit_step(model, weights):
+    """the step's logits against the plain form.  Both round at the same points, so they differ where a sum of another order falls on the other side
+    of a rounding: one step of bf16, 2^-7 of the value, where it does.  A layer has five such points in a row (qkv, attention, h, the gated product,
+    x), the head one more; errors of a layer pass through the next with a gain of about one (the residual stream is normed): 16 * 2^-7 at the very
+    worst, were every value of every point to fall apart; flips are rare and independent, a hundredth of them: 16 * 2^-7 / 10 for the norm."""
+    dec = decoder(model, weights=weights, kv_cache="e4m3")
+    inputs = prompt(150, seed=8)
+    dec.generate(max_new_tokens=3, **inputs)
+    st = next(iter(dec._static.values()))
+    for step, token in ((150, 77), (152, 1234)):
+        st["step"].fill_(step), st["token"].fill_(token)
+        got = dec._step_low_bit(st).to(F64)
+        want, rows = plain_step(dec, st)
+        err = float((got - want).norm() / want.norm())
+        print(f"[parity] low-bit step ({weights}): logits off by {err:.2e}")
+        assert err <= 16 * 2.0 ** -7 / 10
+        for l, (kq, ks, vq, vs) in enumerate(rows):          # the rows that the step wrote: the same up to the flips of their inputs
+            c = st["cache"][l]
+            k, v = (t[0, :, step].to(F64) * s[0, :, step, None].to(F64) for t, s in
+                    ((c.k, c.k_scale), (c.v.reshape(1, 4, -1, 128), c.v_scale)))
+            for a, b in ((k, kq.to(F64) * ks[:, None].to(F64)), (v, vq.to(F64) * vs[:, None].to(F64))):
+                assert (a - b).norm() <= 2.0 ** -5 * b.norm()        # e4m3's own half step is 2^-4; a flip of it here and there
+
+
+@pytest.mark.parametrize("weights", ["bf16", "w4"])
+def test_low_bit_decode_is_its_own_steps(model, config, weights):
+    """the captured step, replayed, gives the tokens of the same step run eagerly; another prompt and a repetition penalty reuse and re-capture it"""
+    dec = decoder(model, weights=weights, kv_cache="e4m3")
+
+    def eager(n, Lp, first):
+        st = next(iter(dec._static.values()))
+        st["step"].fill_(Lp), st["token"].fill_(first)
+        for _ in range(n - 1):
+            dec._step(st)
+        return [first] + st["out_ids"][Lp:Lp + n - 1].tolist()
+    for Lp, seed in ((61, 1), (64, 2), (130, 5)):
+        inputs = prompt(Lp, seed)
+        toks = dec.generate(max_new_tokens=20, **inputs)[0, Lp:].tolist()
+        assert toks == eager(20, Lp, toks[0])
+    assert dec.captures == 1
+    config.repetition_penalty = 1.2
+    inputs = prompt(70, 6)
+    toks = dec.generate(max_new_tokens=20, **inputs)[0, 70:].tolist()
+    assert len(set(toks)) > 1 and dec.captures == 2
+    assert toks == dec.generate(max_new_tokens=20, **inputs)[0, 70:].tolist() and dec.captures == 2
+
+
+def test_four_bit_copies_follow_the_weights(model):
+    """a weight changed in place, moved, or changed through .data with reset(): new copies and a new capture; nothing otherwise"""
+    dec = decoder(model, weights="w4", kv_cache="e4m3")
+    inputs = prompt(40, 9)
+    a = dec.generate(max_new_tokens=10, **inputs)
+    copies = dec._w4
+    assert torch.equal(dec.generate(max_new_tokens=10, **inputs), a) and dec._w4 is copies
+    head = model.lm_head.weight
+    kept = head.detach().clone()
+    try:
+        with torch.no_grad():
+            head.copy_(kept.roll(7, 0))
+        b = dec.generate(max_new_tokens=10, **inputs)
+        assert dec._w4 is not copies and int(b[0, 40]) == (int(a[0, 40]) + 7) % 4001
+        head.data.copy_(kept)
+        dec.reset()
+        assert torch.equal(dec.generate(max_new_tokens=10, **inputs), a)
+    finally:
+        with torch.no_grad():
+            head.copy_(kept)
+
+
+def test_low_bit_choices_are_checked(model):
+    for kw in (dict(weights="w4", kv_cache="bf16"), dict(weights="int8"), dict(kv_cache="fp8"), dict(weights="w4", kv_cache="e4m3", w4_group=1024)):
+        with pytest.raises(ValueError):
+            decoder(model, **kw)
+
+
+def test_a_tree_of_drafts_equals_its_branches(model):
+    """the operators in a speculative step: four drafted tokens as a tree over a cache give each branch what decoding it token by token gives"""
+    from physicedit_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(31)
+    rnd = lambda *s: torch.randn(s, generator=g, device="cuda").to(BF)
+    n, cos = 100, torch.rand((256, 128), generator=g, device="cuda").to(BF)
+    sin = torch.rand((256, 128), generator=g, device="cuda").to(BF)
+    ctx = rnd(1, n, 4, 128), rnd(1, n, 4, 128)
+    q, k, v = rnd(1, 4, 28, 128), rnd(1, 4, 4, 128), rnd(1, 4, 4, 128)
+    parent, depth = [None, 0, 0, 1], [0, 1, 1, 2]                    # 0 -> (1 -> 3, 2)
+    start, zero = torch.tensor([n], dtype=torch.int32, device="cuda"), torch.zeros((1,), dtype=torch.int32, device="cuda")
+    cache = ops.KVCacheE4M3(1, 4, 192, 128)
+    ops.kv_append_e4m3(cache, *ctx, zero)
+    pos = torch.tensor([[n + d for d in depth]], dtype=torch.int32, device="cuda")
+    words = [1, 3, 5, 11]
+    qr = ops.kv_append_e4m3(cache, k, v, start, q=q, cos=cos, sin=sin, positions=pos)
+    got = ops.kv_attention_e4m3(qr, cache, start, tree=torch.tensor([words], device="cuda"))
+    for leaf in (2, 3):
+        path = []
+        i = leaf
+        while i is not None:
+            path.insert(0, i)
+            i = parent[i]
+        line = ops.KVCacheE4M3(1, 4, 192, 128)
+        ops.kv_append_e4m3(line, *ctx, zero)
+        for t, i in enumerate(path):
+            at = start + t
+            one = ops.kv_append_e4m3(line, k[:, i:i + 1], v[:, i:i + 1], at, q=q[:, i:i + 1], cos=cos, sin=sin)
+            alone = ops.kv_attention_e4m3(one, line, at)
+            assert torch.equal(one[0, 0], qr[0, i])
+            # the same numbers in another order of sums, each rounded once: half a step apart on either side
+            assert ((got[0, i].float() - alone[0, 0].float()).abs() <= 2.0 ** -7 * alone[0, 0].float().abs() + 2.0 ** -14).all()
