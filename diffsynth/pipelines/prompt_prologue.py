@@ -332,10 +332,11 @@ class GraphDecoder:
     the patched `generate()` produces.  EOS is tested on the host every `chunk` tokens; the overshoot is discarded.
 
     Low-bit decode (opt-in; the prefill stays bf16): kv_cache="e4m3" keeps keys and values as e4m3 codes with a scale per token and head
-    (pe_kv_append_e4m3 quantises them as they are written, pe_kv_attention_e4m3 reads them back: half the cache bytes), weights="w4" also runs
-    every linear of the step on 4-bit weights with a scale and zero point per output and `w4_group` inputs (pe_gemv_w4: a quarter of the weight
-    bytes; q / k / v and gate / up are one matrix each, the RMSNorm weights folded into their columns).  The 4-bit copies are made at the first
-    call from the model's weights and again when those move or change (call reset() after changing them through `.data`).
+    (pe_kv_append_e4m3 quantises them as they are written, pe_kv_attention_e4m3 reads them back: half the cache bytes; the step keeps q / k / v of
+    a layer as one more matrix), weights="w4" also runs every linear of the step on 4-bit weights with a scale and zero point per output and
+    `w4_group` inputs (pe_gemv_w4: a quarter of the weight bytes; q / k / v and gate / up are one matrix each, the RMSNorm weights folded into
+    their columns).  The copies are made at the first call from the model's weights and again when those move or change (call reset() after
+    changing them through `.data`).
     Penalties and masks: a repetition_penalty or suppress_tokens of the generation config, or generate(prefix_allowed_tokens_fn=), make the
     next token the first maximum of the processed scores (pe_select_token) instead of the plain arg-max."""
 
@@ -392,21 +393,23 @@ class GraphDecoder:
             at, mlp = ly.self_attn, ly.mlp
             ts += [at.q_proj.weight, at.q_proj.bias, at.k_proj.weight, at.k_proj.bias, at.v_proj.weight, at.v_proj.bias, at.o_proj.weight,
                    mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight, ly.input_layernorm.weight, ly.post_attention_layernorm.weight]
-        # the 4-bit copies hold the weights' values, not their addresses alone: the version counts changes in place
-        version = (lambda t: t._version if not t.is_inference() else 0) if self.weights == "w4" else (lambda t: 0)
+        # the low-bit step's copies hold the weights' values, not their addresses alone: the version counts changes in place
+        version = (lambda t: t._version if not t.is_inference() else 0) if self.kv_cache == "e4m3" else (lambda t: 0)
         return tuple((t.data_ptr(), t.dtype, tuple(t.shape), version(t)) if t is not None else None for t in ts)
 
     def reset(self):
-        """Drop the captured graph and its static planes (28 KiB per cache row) and the 4-bit weight copies now instead of at the next call.
+        """Drop the captured graph and its static planes (28 KiB per cache row) and the low-bit step's weight copies now instead of at the next call.
         Nothing has to call this for correctness: generate() notices moved / re-allocated weights by itself (_weights_fingerprint) and captures
-        again -- except for weights="w4" after a change through `.data`, which nothing records."""
+        again -- except in the low-bit step after a change through `.data`, which nothing records."""
         self._static = {}
         self._w4 = None
 
     def _packed(self, fp):
-        """the 4-bit copies of the weights that `fp` describes: per layer (qkv, its bias, o, gate_up, down), and the lm_head"""
+        """the copies that the low-bit step keeps of the weights `fp` describes: per layer q / k / v as one matrix and its bias and, for "w4", all in
+        4 bits: (qkv, its bias, o, gate_up, down), and the lm_head"""
         if self._w4 is None or self._w4[0] != fp:
             self._w4 = None                                # the old copies go before the new ones come
+            w4 = self.weights == "w4"
             q4 = lambda w, norm=None: self.ops.quantize_w4(w.contiguous(), self.w4_group, norm_w=norm)
             layers = []
             for ly in self.layers:
@@ -415,10 +418,11 @@ class GraphDecoder:
                 if any(b is None for b in bias):
                     bias = [torch.zeros(p.out_features, dtype=p.weight.dtype, device=p.weight.device) if p.bias is None else p.bias
                             for p in (at.q_proj, at.k_proj, at.v_proj)]
-                layers.append((q4(torch.cat([at.q_proj.weight, at.k_proj.weight, at.v_proj.weight]), ly.input_layernorm.weight), torch.cat(bias),
-                               q4(at.o_proj.weight), q4(torch.cat([mlp.gate_proj.weight, mlp.up_proj.weight]), ly.post_attention_layernorm.weight),
-                               q4(mlp.down_proj.weight)))
-            self._w4 = (fp, layers, q4(self.model.lm_head.weight, self.lm.norm.weight))
+                qkv = torch.cat([at.q_proj.weight, at.k_proj.weight, at.v_proj.weight])
+                layers.append((q4(qkv, ly.input_layernorm.weight), torch.cat(bias), q4(at.o_proj.weight),
+                               q4(torch.cat([mlp.gate_proj.weight, mlp.up_proj.weight]), ly.post_attention_layernorm.weight),
+                               q4(mlp.down_proj.weight)) if w4 else (qkv, torch.cat(bias)))
+            self._w4 = (fp, layers, q4(self.model.lm_head.weight, self.lm.norm.weight) if w4 else None)
         return self._w4
 
     def _step_low_bit(self, st):
@@ -430,11 +434,13 @@ class GraphDecoder:
             at, mlp = ly.self_attn, ly.mlp
             n1, n2 = ly.input_layernorm, ly.post_attention_layernorm
             e1, e2 = float(n1.variance_epsilon), float(n2.variance_epsilon)
+            w_qkv, b_qkv, *w_more = st["w4"][1][l]
             if self.weights == "w4":
-                w_qkv, b_qkv, w_o, w_gu, w_down = st["w4"][1][l]
-                q, k, v = ops.gemv_w4(x, w_qkv, bias=b_qkv, norm_eps=e1).view(1, 1, -1, 128).split([nq, self.hkv, self.hkv], dim=2)
+                w_o, w_gu, w_down = w_more
+                qkv = ops.gemv_w4(x, w_qkv, bias=b_qkv, norm_eps=e1)
             else:
-                q, k, v = (ops.gemv_norm(x, n1.weight, e1, p.weight, p.bias).view(1, 1, -1, 128) for p in (at.q_proj, at.k_proj, at.v_proj))
+                qkv = ops.gemv_norm(x, n1.weight, e1, w_qkv, b_qkv)
+            q, k, v = qkv.view(1, 1, -1, 128).split([nq, self.hkv, self.hkv], dim=2)
             cache = st["cache"][l]
             q = ops.kv_append_e4m3(cache, k, v, st["step"], q=q, cos=st["cos"], sin=st["sin"])
             a = ops.kv_attention_e4m3(q, cache, st["step"], scale=float(at.scaling)).view(-1)
@@ -537,7 +543,6 @@ class GraphDecoder:
             st["vc"] = torch.zeros_like(st["kc"])
             if self.kv_cache == "e4m3":
                 st["cache"] = [self.ops.KVCacheE4M3(1, self.hkv, bucket, 128, device=dev) for _ in range(L)]
-            if self.weights == "w4":
                 st["w4"] = self._packed(fp)
             if self.split_attention and self.kv_cache == "bf16":     # scratch of the three-launch single-query attention (layers run one after the other: one buffer)
                 st["attn_ws"] = self.ops.decode_attention_workspace(len(self.layers[0].self_attn.q_proj.weight) // 128, bucket, dev)
