@@ -339,11 +339,11 @@ __global__ void __launch_bounds__(WR * WK * 64, 2) kv_attention_kernel(KvAttenti
     float m = -INFINITY, l = 0.f;                                            // running maximum of the scores (times log2 e) and sum
 
     auto work = [&](Block& t, int blk) __attribute__((always_inline)) {
-        f32x4 s4[4] = {};
+        f32x4 s4[4] = {};                         // four independent accumulators in turn: an MFMA's result is not there for the next one
 #pragma unroll
-        for (int h = 0; h < 4; ++h)
+        for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
+            for (int h = 0; h < 4; ++h)
                 s4[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes8(t.k[h][s >> 1][2 * (s & 1)], t.k[h][s >> 1][2 * (s & 1) + 1]), qf[s], s4[h], 0, 0, 0);
 #pragma unroll
         for (int h = 0; h < 4; ++h)
@@ -365,10 +365,10 @@ __global__ void __launch_bounds__(WR * WK * 64, 2) kv_attention_kernel(KvAttenti
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, s4[h][i]);
         top = max_over_j(top);
-        const float m_new = fmaxf(m, top);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        if (__any(m_new > m)) {
-            const float alpha = __builtin_amdgcn_exp2f(m - m_use);       // 0 from -inf
+        // the reference of the exponentials follows the maximum only when it falls 2^8 behind: probabilities up to 256 cost nothing in fp32, the rescaling does
+        if (__any(top > m + 8.f)) {
+            const float m_new = fmaxf(m, top);
+            const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m_new);        // 0 from -inf
             l *= alpha;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
@@ -376,26 +376,32 @@ __global__ void __launch_bounds__(WR * WK * 64, 2) kv_attention_kernel(KvAttenti
                 for (int i = 0; i < 4; ++i) o[dt][i] *= alpha;
             m = m_new;
         }
-        bf16x8 ph[2], pl[2];
+        const float m_use = m == -INFINITY ? 0.f : m;
+        u32x4 ph[2], pl[2];                       // p * scale_v as its upper 16 bits (a bf16) and the rest, rounded to bf16
 #pragma unroll
         for (int h = 0; h < 4; ++h)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float p = __builtin_amdgcn_exp2f(s4[h][i] - m_use);
-                l += p;
-                const float pv = p * t.vs[h][i];
-                const bf16 top8 = (bf16)pv;
-                ph[h >> 1][4 * (h & 1) + i] = top8;
-                pl[h >> 1][4 * (h & 1) + i] = (bf16)(pv - (float)top8);
+            for (int i = 0; i < 4; i += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(s4[h][i] - m_use), p1 = __builtin_amdgcn_exp2f(s4[h][i + 1] - m_use);
+                l += p0 + p1;
+                const float w0 = p0 * t.vs[h][i], w1 = p1 * t.vs[h][i + 1];
+                const uint32_t u0 = __float_as_uint(w0), u1 = __float_as_uint(w1);
+                typedef __attribute__((ext_vector_type(2))) __bf16 v2;
+                const v2 rest = {(bf16)(w0 - __uint_as_float(u0 & 0xffff0000u)), (bf16)(w1 - __uint_as_float(u1 & 0xffff0000u))};
+                ph[h >> 1][2 * (h & 1) + (i >> 1)] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
+                pl[h >> 1][2 * (h & 1) + (i >> 1)] = __builtin_bit_cast(uint32_t, rest);
             }
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+        for (int s = 0; s < 2; ++s) {
+            bf16x8 f[DT];
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const bf16x8 f = codes8(t.v[dt][2 * s], t.v[dt][2 * s + 1]);
-                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, ph[s], o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, pl[s], o[dt], 0, 0, 0);
+            for (int dt = 0; dt < DT; ++dt) {
+                f[dt] = codes8(t.v[dt][2 * s], t.v[dt][2 * s + 1]);
+                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[dt], __builtin_bit_cast(bf16x8, ph[s]), o[dt], 0, 0, 0);
             }
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[dt], __builtin_bit_cast(bf16x8, pl[s]), o[dt], 0, 0, 0);
+        }
     };
     if (SHARED) {
         // every wave takes part in every step: the barrier at its top says that this block is there and that the one before is done with.  The next block

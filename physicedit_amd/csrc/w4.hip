@@ -216,7 +216,10 @@ int launch_gemv_w4(const W4Problem& p, hipStream_t stream) {
     // 33: 19.1 and 13.1), from three on its chunks fill the LDS (60 rows, N = 12001: 2, 8 18.1 us, 2, 4 15.0, 4, 4 17.3; 64 rows, N = 152064: 199, 179, 202).
     const int tiles = (p.N + 15) / 16, mt = (p.M + 15) / 16;
     const int size = tiles <= 256 ? 0 : tiles <= (mt >= 3 ? 512 : 1024) ? 1 : 2;
+    // The gated epilogue works on pairs of tiles: with many, one pair and four waves for few rows (N = 37888, one row: 2, 4 18.4 us, 4, 8 19.7; 16 rows: 22.0, 21.3).
 #define PE_W4(MT, R, W) { if (p.swiglu) w4_launch<MT, (R == 1 ? 2 : R), (R == 1 ? 8 : W), true>(a, gs, p.norm, stream); else w4_launch<MT, R, W, false>(a, gs, p.norm, stream); }
+    if (p.swiglu && size == 2 && p.M <= 8) w4_launch<1, 2, 4, true>(a, gs, p.norm, stream);
+    else
     if (mt == 1) { if (size == 0) PE_W4(1, 1, 16) else if (size == 1) PE_W4(1, 1, 8) else PE_W4(1, 4, 8) }
     else if (mt == 2) { if (size == 0) PE_W4(2, 1, 8) else if (size == 1) PE_W4(2, 2, 8) else PE_W4(2, 4, 8) }
     else if (mt == 3) { if (size == 0) PE_W4(3, 1, 8) else if (size == 1) PE_W4(3, 2, 8) else PE_W4(3, 2, 4) }
