@@ -492,9 +492,12 @@ class GraphDecoder:
         V = st["counts"].shape[1]
         bits = torch.full((V + 31,), ids is None, dtype=torch.bool)
         if ids is not None:
-            bits[torch.as_tensor(ids, dtype=torch.long)] = True
-        if getattr(self.model.generation_config, "suppress_tokens", None):
-            bits[torch.as_tensor(list(self.model.generation_config.suppress_tokens), dtype=torch.long)] = False
+            ids = torch.as_tensor(ids, dtype=torch.long).cpu()
+            if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= V):
+                raise ValueError(f"prefix_allowed_tokens_fn: token ids outside 0 ... {V - 1}")
+            bits[ids] = True
+        gone = [t for t in (getattr(self.model.generation_config, "suppress_tokens", None) or ()) if 0 <= t < V]
+        bits[torch.as_tensor(gone, dtype=torch.long)] = False
         words = (bits[:V + (-V) % 32].view(-1, 32).long() << torch.arange(32)).sum(1)
         st["allowed"].copy_(torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32))
 

@@ -311,7 +311,7 @@ typedef struct pe_w4_weight {
 } pe_w4_weight;
 /* out[M, N] = r * (x @ W^T) + bias + res for 1 ... 64 rows x [M,K] bf16 (finite values; row stride ldx, a multiple of 8; 16-byte aligned).  norm_eps >= 0:
  * r[m] = rsqrt(mean(x[m]^2) + norm_eps), an RMSNorm whose weight the caller folded into W; norm_eps < 0: r = 1.  bias [N], res [M, N] (row
- * stride ldr; may be out itself) nullable.  swiglu != 0: W holds the F = N / 2 gate rows, then the F up rows (F % 16 == 0), and
+ * stride ldr; may be out itself) nullable; out may not be x.  swiglu != 0: W holds the F = N / 2 gate rows, then the F up rows (F % 16 == 0), and
  * out[M, F] = silu(gate) * up (no res). */
 int pe_gemv_w4(const void* x, long long ldx, int M, const pe_w4_weight* w, const void* bias, const void* res, long long ldr, void* out,
                long long ldo, int swiglu, float norm_eps, void* stream);

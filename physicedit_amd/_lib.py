@@ -268,6 +268,31 @@ def lib() -> C.CDLL:
     return _lib
 
 
+_binding = None
+
+
+def binding():
+    """The native Python binding of the low-bit operators (csrc/binding.cpp), bound to lib()'s entry points.  No fallback: a missing or stale
+    module raises."""
+    global _binding
+    if _binding is None:
+        import torch
+        from . import build
+        try:
+            from . import _binding as module
+        except ImportError as e:
+            raise PeError(f"{build.BINDING} cannot be loaded ({e}): build it with `python -m physicedit_amd.build`") from e
+        if module.build_id != build.binding_id():
+            raise PeError(f"{build.BINDING} is stale (another source, header or torch version): run `python -m physicedit_amd.build`")
+        handle = lib()
+        names = ("pe_last_error", "pe_gemv_w4", "pe_kv_append_e4m3", "pe_kv_attention_workspace_bytes", "pe_kv_attention_e4m3", "pe_process_logits",
+                 "pe_select_token_workspace_bytes", "pe_select_token", "pe_token_counts_add")
+        module.bind(tuple(C.cast(getattr(handle, n), c_void_p).value for n in names), torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream,
+                    PeError, torch.OutOfMemoryError)
+        _binding = module
+    return _binding
+
+
 def check(rc: int, what: str = "") -> None:
     if rc != 0:
         msg = lib().pe_last_error().decode("utf-8", "replace")

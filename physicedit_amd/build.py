@@ -1,4 +1,4 @@
-"""Build libphysicedit_amd.so (gfx950 only) in-tree with hipcc.
+"""Build libphysicedit_amd.so (gfx950 only) in-tree with hipcc, and _binding.so, the native Python binding of the low-bit operators, with g++.
 
     python -m physicedit_amd.build [--force]
 
@@ -55,6 +55,43 @@ def source_hash() -> str:
     return hh.hexdigest()[:16]
 
 
+BINDING_SRC = os.path.join(CSRC, "binding.cpp")
+BINDING = os.path.join(HERE, "_binding.so")
+
+
+def binding_id() -> str:
+    """what _binding.so was built from and against: its source, the C header and the torch version (the module links to torch's C++ ABI)"""
+    import hashlib
+    import torch
+    hh = hashlib.sha256(torch.__version__.encode())
+    for path in (BINDING_SRC, os.path.join(CSRC, "..", "..", "include", "physicedit_amd.h")):
+        with open(path, "rb") as f:
+            hh.update(f.read())
+    return hh.hexdigest()[:16]
+
+
+def build_binding(force: bool = False, verbose: bool = True) -> str:
+    import sysconfig
+    import torch
+    ident, stamp = binding_id(), os.path.join(OBJ, "binding_id.txt")
+    os.makedirs(OBJ, exist_ok=True)
+    if not force and os.path.exists(BINDING) and os.path.exists(stamp) and open(stamp).read().strip() == ident:
+        return BINDING
+    if verbose:
+        print("[physicedit_amd.build] compiling the Python binding ...", flush=True)
+    root = os.path.dirname(torch.__file__)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", f'-DPE_BINDING_ID="{ident}"',
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + os.path.join(root, "include"),
+           "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"), "-I" + sysconfig.get_paths()["include"], BINDING_SRC, "-o", BINDING,
+           "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDING_SRC}:\n{r.stdout}\n{r.stderr}")
+    with open(stamp, "w") as f:
+        f.write(ident)
+    return BINDING
+
+
 def _stale(target: str, deps) -> bool:
     if not os.path.exists(target):
         return True
@@ -104,6 +141,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         if verbose:
             print(f"[physicedit_amd.build] linked {LIB}", flush=True)
+    build_binding(force, verbose)
     return LIB
 
 

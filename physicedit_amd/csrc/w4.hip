@@ -200,6 +200,7 @@ int launch_gemv_w4(const W4Problem& p, hipStream_t stream) {
     const int cols = p.swiglu ? p.N / 2 : p.N;
     PE_REQUIRE(!p.swiglu || p.N % 32 == 0, "gemv_w4: the gated epilogue needs a multiple of 16 gate and up rows (N=%d)", p.N);
     PE_REQUIRE(!(p.swiglu && p.res), "gemv_w4: no residual with the gated epilogue");
+    PE_REQUIRE(p.out != p.x, "gemv_w4: out may be res, not x (every work-group reads all of x)");
     PE_REQUIRE(p.ldo >= cols && (!p.res || p.ldr >= cols), "gemv_w4: row stride below the %d columns", cols);
     PE_REQUIRE(!p.norm || p.eps >= 0.f, "gemv_w4: negative eps");
     W4Args a;

@@ -6,14 +6,13 @@ host.  These are what the `-m gpu` parity tests call, and what `physicedit_amd.d
 from __future__ import annotations
 
 import ctypes as C
-import functools
 import math
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import check, lib, stream_ptr
+from ._lib import binding as _binding, check, lib, stream_ptr
 
 BF = torch.bfloat16
 EPI = {"bias": 0, "gelu_sigmoid": 1, "gelu_erf": 2, "gate_res": 3, "silu": 5}
@@ -501,18 +500,14 @@ def sdpa_heads64(q: torch.Tensor, kv: torch.Tensor, heads: int) -> torch.Tensor:
 
 
 # ---- the low-bit decode step: 4-bit linears, the e4m3 key/value cache, next-token scores (include/physicedit_amd.h) -----------------
-# These are called once per token and layer by programs that do not capture the step, so the checks read each tensor attribute once (an attribute
-# costs about as much as passing an argument) and the launch asks for the raw stream of the current device.
-_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
-
-
+# Their checks, allocations and launches are in csrc/binding.cpp (_lib.binding()); laying a weight out is here.
 def _stream_of(dev: int, name: str) -> int:
     """the current stream of device `dev`, which has to be the current device"""
     if dev < 0:
         raise ValueError(f"{name}: expected a CUDA/HIP tensor (physicedit_amd has no CPU path)")
-    if dev != _device():
-        raise ValueError(f"{name}: on cuda:{dev}, but the current device is cuda:{_device()} (torch.cuda.device(...))")
-    return _raw_stream(dev)
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"{name}: on cuda:{dev}, but the current device is cuda:{torch.cuda.current_device()} (torch.cuda.device(...))")
+    return stream_ptr()
 
 
 def _at(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, shape, dev: int) -> Optional[int]:
@@ -531,7 +526,7 @@ class W4Weight:
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor, N: int, K: int, group: int):
         self.codes, self.scale, self.N, self.K, self.group = codes, scale, N, K, group
         self._c = _lib.W4Weight(codes.data_ptr(), scale.data_ptr(), N, K, group)
-        self._ref, self._dev = C.byref(self._c), codes.get_device()
+        self._addr, self._dev = C.addressof(self._c), codes.get_device()
 
     @property
     def nbytes(self) -> int:
@@ -601,31 +596,11 @@ def gemv_w4(x: torch.Tensor, w: W4Weight, bias: Optional[torch.Tensor] = None, r
             norm_eps: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [M, K] or [K] (M <= 64 rows; a row stride is fine) @ w.T + bias + res -> [M, N] or [N], one rounding.  epilogue="swiglu": w holds the gate
     rows, then as many up rows (a multiple of 16): silu(gate) * up.  norm_eps: x is RMS-normalised (its norm weight folded into w)."""
-    swiglu = epilogue == "swiglu"
-    if not swiglu and epilogue != "bias":
+    if epilogue != "bias" and epilogue != "swiglu":
         raise ValueError(f"gemv_w4: epilogue {epilogue!r} ('bias' or 'swiglu')")
-    if norm_eps is None:
-        norm_eps = -1.0
-    elif not norm_eps >= 0:
+    if norm_eps is not None and not norm_eps >= 0:
         raise ValueError(f"gemv_w4: norm_eps={norm_eps}")
-    dev, K, cols = w._dev, w.K, w.N // 2 if swiglu else w.N
-    stream = _stream_of(dev, "w")
-    rows, strides = x.shape, x.stride()
-    n = len(rows)
-    if x.dtype is not BF or n not in (1, 2) or rows[-1] != K or strides[-1] != 1 or x.get_device() != dev:
-        raise ValueError(f"gemv_w4: expected bf16 rows of {K} contiguous values on cuda:{dev}, got {x.dtype} {tuple(rows)} on {x.device}")
-    M = 1 if n == 1 else rows[0]
-    shape = (cols,) if n == 1 else (M, cols)
-    if out is None:
-        out = x.new_empty(shape)
-        to = out.data_ptr()
-    else:
-        to = _at(out, "out", BF, shape, dev)
-    rc = lib().pe_gemv_w4(x.data_ptr(), strides[0] if M > 1 else K, M, w._ref, _at(bias, "bias", BF, (w.N,), dev), _at(res, "res", BF, shape, dev), cols,
-                          to, cols, swiglu, norm_eps, stream)
-    if rc:
-        check(rc, "pe_gemv_w4")
-    return out
+    return _binding().gemv_w4(x, w._addr, w._dev, bias, res, epilogue == "swiglu", -1.0 if norm_eps is None else norm_eps, out)
 
 
 class KVCacheE4M3:
@@ -642,22 +617,9 @@ class KVCacheE4M3:
         self.k_scale = torch.zeros((batch, n_kv, capacity), dtype=torch.float32, device=device)
         self.v_scale = torch.zeros_like(self.k_scale)
         self._c = _lib.KvCache(self._k.data_ptr(), self._v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), batch, n_kv, capacity, head_dim)
-        self._ref, self._dev = C.byref(self._c), self._k.get_device()
+        self._addr, self._dev = C.addressof(self._c), self._k.get_device()
         self.k = self._k.view(F8)
         self.v = self._v.view(F8).transpose(3, 4)
-
-
-def _heads(t: torch.Tensor, name: str, shape, dev: int):
-    """address and strides (batch, token, head) of a bf16 [batch, T, heads, D] tensor with contiguous channels and rows of whole 16 bytes; a
-    dimension of one entry has any stride"""
-    st, at = t.stride(), t.data_ptr()
-    if t.dtype is not BF or t.shape != shape or st[3] != 1 or t.get_device() != dev:
-        raise ValueError(f"{name}: expected bf16 {tuple(shape)} with contiguous channels on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if (st[0] | st[1] | st[2]) & 7:
-        st = tuple(0 if shape[i] == 1 else st[i] for i in range(3))
-    if at & 15 or (st[0] | st[1] | st[2]) & 7:
-        raise ValueError(f"{name}: rows must be 16-byte aligned (strides {t.stride()})")
-    return at, st[:3]
 
 
 def kv_append_e4m3(cache: KVCacheE4M3, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, q: Optional[torch.Tensor] = None,
@@ -666,49 +628,12 @@ def kv_append_e4m3(cache: KVCacheE4M3, k: torch.Tensor, v: torch.Tensor, start: 
     """k, v [batch, T, n_kv, D] (any strides of whole 16 bytes) into rows start[b] ... start[b] + T - 1 (int32 [batch], device) of the cache.  cos, sin
     [rows, D] (bf16 or fp32): k -- and q [batch, T, n_q, D], returned rotated, contiguous -- are rotated with table row positions[b, t] (int32;
     default start[b] + t) first.  Rows past the capacity and sequences with start < 0 are not written (their q comes back zero)."""
-    dev, B, H, D = cache._dev, cache.batch, cache.n_kv, cache.head_dim
-    stream = _stream_of(dev, "cache")
-    if k.dim() != 4:
-        raise ValueError(f"k: expected [batch, T, n_kv, D], got {tuple(k.shape)}")
-    T = k.shape[1]
-    (ka, ks), (va, vs) = _heads(k, "k", (B, T, H, D), dev), _heads(v, "v", (B, T, H, D), dev)
-    qa, qs, qo, n_q, ca, sa, rows, f32 = None, (0, 0, 0), None, 0, None, None, 0, 0
-    if cos is not None and sin is not None:
-        kind, (rows, _) = cos.dtype, cos.shape
-        f32 = kind is torch.float32
-        if not f32 and kind is not BF:
-            raise ValueError(f"cos: expected bf16 or fp32, got {kind}")
-        ca, sa = _at(cos, "cos", kind, (rows, D), dev), _at(sin, "sin", kind, (rows, D), dev)
-    elif cos is not None or sin is not None or q is not None or positions is not None:
-        raise ValueError("kv_append_e4m3: q and positions need cos and sin, which come together")
-    if q is not None:
-        if q.dim() != 4:
-            raise ValueError(f"q: expected [batch, T, n_q, D], got {tuple(q.shape)}")
-        n_q = q.shape[2]
-        shape = (B, T, n_q, D)
-        qa, qs = _heads(q, "q", shape, dev)
-        if out is None:
-            out = q.new_empty(shape)
-        qo = _at(out, "out", BF, shape, dev)
-    a = _lib.KvAppendArgs(qa, ka, va, qs, ks, vs, qo, ca, sa, rows, f32, _at(positions, "positions", torch.int32, (B, T), dev),
-                          _at(start, "start", torch.int32, (B,), dev), T, n_q)
-    rc = lib().pe_kv_append_e4m3(cache._ref, C.byref(a), stream)
-    if rc:
-        check(rc, "pe_kv_append_e4m3")
-    return out if q is not None else None
-
-
-@functools.lru_cache(maxsize=256)
-def _kv_workspace_bytes(batch: int, n_kv: int, T: int, n_q: int, head_dim: int, capacity: int) -> int:
-    return lib().pe_kv_attention_workspace_bytes(batch, n_kv, T, n_q, head_dim, capacity)
-
-
-_Strides = C.c_longlong * 3
+    return _binding().kv_append_e4m3(cache._addr, cache._dev, k, v, start, q, cos, sin, positions, out)
 
 
 def kv_attention_workspace(cache: KVCacheE4M3, T: int, n_q: int) -> torch.Tensor:
     """scratch of kv_attention_e4m3 for calls that want to keep one (one per stream)"""
-    return cache._k.new_empty((_kv_workspace_bytes(cache.batch, cache.n_kv, T, n_q, cache.head_dim, cache.capacity),))
+    return cache._k.new_empty((lib().pe_kv_attention_workspace_bytes(cache.batch, cache.n_kv, T, n_q, cache.head_dim, cache.capacity),))
 
 
 def kv_attention_e4m3(q: torch.Tensor, cache: KVCacheE4M3, start: torch.Tensor, tree: Optional[torch.Tensor] = None, scale: Optional[float] = None,
@@ -716,51 +641,7 @@ def kv_attention_e4m3(q: torch.Tensor, cache: KVCacheE4M3, start: torch.Tensor, 
     """Attention of the T <= 64 newest tokens, appended at rows start[b] + t: q [batch, T, n_q, D] -> [batch, T, n_q * D].  Token t sees the cache rows
     below start[b] and new token j where bit j of tree[b, t] (int64) is set; tree None: causal.  scale: default 1 / sqrt(D).  A query that sees
     nothing gives zeros."""
-    dev, B, D = cache._dev, cache.batch, cache.head_dim
-    stream = _stream_of(dev, "cache")
-    if q.dim() != 4:
-        raise ValueError(f"q: expected [batch, T, n_q, D], got {tuple(q.shape)}")
-    _, T, n_q, _ = q.shape
-    qa, qs = _heads(q, "q", (B, T, n_q, D), dev)
-    if not 1 <= T <= 64 or n_q % cache.n_kv or n_q < 1:
-        raise ValueError(f"kv_attention_e4m3: {T} new tokens (1 ... 64), {n_q} query heads over {cache.n_kv} kv heads")
-    if out is None:
-        out = q.new_empty((B, T, n_q * D))
-        to = out.data_ptr()
-    else:
-        to = _at(out, "out", BF, (B, T, n_q * D), dev)
-    if workspace is None:
-        workspace = kv_attention_workspace(cache, T, n_q)
-    elif workspace.get_device() != dev or not workspace.is_contiguous():
-        raise ValueError(f"workspace: expected a contiguous tensor on cuda:{dev}")
-    rc = lib().pe_kv_attention_e4m3(cache._ref, qa, _Strides(*qs), _at(start, "start", torch.int32, (B,), dev), _at(tree, "tree", torch.int64, (B, T), dev),
-                                    T, n_q, D ** -0.5 if scale is None else scale, to, workspace.data_ptr(), workspace.nbytes, stream)
-    if rc:
-        check(rc, "pe_kv_attention_e4m3")
-    return out
-
-
-def _table(t, name, dtype, R: int, n: int, dev: int):
-    """address and row stride of a table that is there once ([n], stride 0) or for every row ([R, n])"""
-    if t is None:
-        return None, 0
-    return (_at(t, name, dtype, (n,), dev), 0) if t.dim() == 1 else (_at(t, name, dtype, (R, n), dev), n)
-
-
-def _logits_args(logits, counts, penalties, bias, allowed):
-    dev = logits.get_device()
-    stream = _stream_of(dev, "logits")
-    kind, shape, strides = logits.dtype, logits.shape, logits.stride()
-    f32 = kind is torch.float32
-    if not f32 and kind is not BF or len(shape) != 2 or strides[1] != 1 and shape[1] > 1 or 0 in shape:
-        raise ValueError(f"logits: expected bf16 or fp32 [rows, vocab] with contiguous rows, got {kind} {tuple(shape)}")
-    R, V = shape
-    if penalties is not None and counts is None:
-        raise ValueError("penalties: they need the counts")
-    pa, pl = _table(penalties, "penalties", torch.float32, R, 3, dev)
-    ba, bl = _table(bias, "bias", torch.float32, R, V, dev)
-    ma, ml = _table(allowed, "allowed", torch.int32, R, (V + 31) // 32, dev)
-    return _lib.LogitsArgs(logits.data_ptr(), strides[0] if R > 1 else V, f32, R, V, _at(counts, "counts", torch.int16, shape, dev), V, pa, pl, ba, bl, ma, ml), R, V, dev, stream
+    return _binding().kv_attention_e4m3(q, cache._addr, cache._dev, start, tree, scale, out, workspace)
 
 
 def process_logits(logits: torch.Tensor, counts: Optional[torch.Tensor] = None, penalties: Optional[torch.Tensor] = None,
@@ -769,18 +650,7 @@ def process_logits(logits: torch.Tensor, counts: Optional[torch.Tensor] = None, 
     counts int16 [rows, vocab]: bit 15 (the value is negative) = the prompt holds the token, the rest = how often it was generated (token_counts_add
     keeps them); penalties fp32 [rows, 3] or [3]: repetition (divides positive, multiplies other scores of seen tokens), presence, frequency; bias fp32
     [vocab] or [rows, vocab]; allowed int32 [rows, ceil(vocab / 32)] or [ceil(vocab / 32)]: token v is bit v % 32 of word v / 32, clear = -inf."""
-    a, R, V, dev, stream = _logits_args(logits, counts, penalties, bias, allowed)
-    if out is None:
-        out = logits.new_empty((R, V), dtype=torch.float32)
-    rc = lib().pe_process_logits(C.byref(a), _at(out, "out", torch.float32, (R, V), dev), stream)
-    if rc:
-        check(rc, "pe_process_logits")
-    return out
-
-
-@functools.lru_cache(maxsize=256)
-def _select_workspace_bytes(rows: int, vocab: int) -> int:
-    return lib().pe_select_token_workspace_bytes(rows, vocab)
+    return _binding().process_logits(logits, counts, penalties, bias, allowed, out)
 
 
 def select_token(logits: torch.Tensor, counts: Optional[torch.Tensor] = None, penalties: Optional[torch.Tensor] = None,
@@ -789,37 +659,10 @@ def select_token(logits: torch.Tensor, counts: Optional[torch.Tensor] = None, pe
                  workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The greedy choice among process_logits' scores, without writing them: int32 [rows], the first maximum (NaN never wins), -1 where everything
     is -inf.  update_counts: counts[row, token] += 1.  step / out_ids (int32, one row): decode_argmax's device-side counter and token list."""
-    a, R, V, dev, stream = _logits_args(logits, counts, penalties, bias, allowed)
-    if update_counts and counts is None:
-        raise ValueError("select_token: update_counts without counts")
-    if out is None:
-        out = logits.new_empty((R,), dtype=torch.int32)
-    ids = at = None
-    room = 0
-    if step is not None or out_ids is not None:
-        if step is None or out_ids is None or R != 1 or step.numel() != 1 or out_ids.dim() != 1 or out_ids.numel() < 1:
-            raise ValueError("select_token: step and out_ids come together, for one row")
-        room = out_ids.numel()
-        ids, at = _at(out_ids, "out_ids", torch.int32, (room,), dev), _at(step, "step", torch.int32, step.shape, dev)
-    if workspace is None:
-        workspace = logits.new_empty((_select_workspace_bytes(R, V),), dtype=torch.uint8)
-    elif workspace.get_device() != dev or not workspace.is_contiguous():
-        raise ValueError(f"workspace: expected a contiguous tensor on cuda:{dev}")
-    rc = lib().pe_select_token(C.byref(a), _at(out, "out", torch.int32, (R,), dev), update_counts, ids, at, room, workspace.data_ptr(), workspace.nbytes,
-                               stream)
-    if rc:
-        check(rc, "pe_select_token")
-    return out
+    return _binding().select_token(logits, counts, penalties, bias, allowed, update_counts, out, out_ids, step, workspace)
 
 
 def token_counts_add(counts: torch.Tensor, tokens: torch.Tensor, prompt: bool = False) -> torch.Tensor:
     """counts int16 [rows, vocab] of process_logits, in place: every id of tokens int32 [rows, n] counts one more (up to 32767), or with prompt=True
     is marked as part of the prompt.  Ids outside the vocabulary (padding: -1) are skipped."""
-    dev = counts.get_device()
-    stream = _stream_of(dev, "counts")
-    if counts.dim() != 2 or counts.numel() == 0 or tokens.dim() != 2 or tokens.shape[1] < 1:
-        raise ValueError(f"token_counts_add: counts [rows, vocab] and tokens [rows, n], got {tuple(counts.shape)} and {tuple(tokens.shape)}")
-    (R, V), n = counts.shape, tokens.shape[1]
-    check(lib().pe_token_counts_add(_at(counts, "counts", torch.int16, (R, V), dev), V, R, V, _at(tokens, "tokens", torch.int32, (R, n), dev), n,
-                                    bool(prompt), stream), "pe_token_counts_add")
-    return counts
+    return _binding().token_counts_add(counts, tokens, prompt)

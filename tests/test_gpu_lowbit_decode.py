@@ -73,7 +73,7 @@ def test_penalties_and_masks_match_generate(model, config):
         want = model.generate(**inputs, max_new_tokens=24, min_new_tokens=24)
     got = dec.generate(max_new_tokens=24, **inputs)
     assert torch.equal(got, want)
-    config.suppress_tokens = sorted(set(want[0, 37:45].tolist()))                 # what it liked best is taken away
+    config.suppress_tokens = sorted(set(want[0, 37:45].tolist())) + [4001, 99999]  # what it liked best is taken away; ids outside are nobody's
     with torch.no_grad():
         want2 = model.generate(**inputs, max_new_tokens=24, min_new_tokens=24)
     got2 = dec.generate(max_new_tokens=24, **inputs)
@@ -92,6 +92,9 @@ def test_penalties_and_masks_match_generate(model, config):
     assert all((b - a) % 2 for a, b in zip(toks, toks[1:])) and dec.captures == 2
     with pytest.raises(RuntimeError, match="no token is allowed"):
         dec.generate(max_new_tokens=4, prefix_allowed_tokens_fn=lambda b, i: [] if i.numel() > 38 else [500], **inputs)
+    for outside in (-1, 4001):
+        with pytest.raises(ValueError, match="outside"):
+            dec.generate(max_new_tokens=4, prefix_allowed_tokens_fn=lambda b, i: [5, outside], **inputs)
     config.repetition_penalty = 1.0
     assert torch.equal(dec.generate(max_new_tokens=24, **inputs), plain)          # and back to the plain arg-max
 

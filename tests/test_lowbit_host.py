@@ -54,14 +54,14 @@ def w4(N=32, K=256, group=128, codes=P, scale=P):
     (dict(N=0), {}, "N=0"), ({}, dict(M=0), "M=0"), ({}, dict(M=65), "M=65"), ({}, dict(x=None), "null"), ({}, dict(out=None), "null"),
     ({}, dict(ldx=248), "aligned"), ({}, dict(ldx=260), "aligned"), ({}, dict(x=P + 8), "aligned"), (dict(codes=P + 4), {}, "unaligned"),
     ({}, dict(ldo=31), "row stride"), ({}, dict(res=P, ldr=31), "row stride"), (dict(N=48), dict(swiglu=1), "gated"), ({}, dict(swiglu=1, res=P), "residual"),
-    (dict(N=1 << 27), dict(ldo=1 << 28), "out of range")])
+    (dict(N=1 << 27), dict(ldo=1 << 28), "out of range"), ({}, dict(out=P), "not x")])
 def test_gemv_w4_refusals(lib, kw, args, text):
-    a = dict(x=P, ldx=256, M=1, bias=None, res=None, ldr=32, out=P, ldo=32, swiglu=0, eps=-1.0) | args
+    a = dict(x=P, ldx=256, M=1, bias=None, res=None, ldr=32, out=2 * P, ldo=32, swiglu=0, eps=-1.0) | args
     refused(lib, lib.pe_gemv_w4(a["x"], a["ldx"], a["M"], C.byref(w4(**kw)), a["bias"], a["res"], a["ldr"], a["out"], a["ldo"], a["swiglu"], a["eps"], None), text)
 
 
 def test_gemv_w4_null_weight(lib):
-    refused(lib, lib.pe_gemv_w4(P, 256, 1, None, None, None, 0, P, 32, 0, -1.0, None), "null weight")
+    refused(lib, lib.pe_gemv_w4(P, 256, 1, None, None, None, 0, 2 * P, 32, 0, -1.0, None), "null weight")
 
 
 def cache(k=P, v=P, ks=P, vs=P, batch=2, n_kv=2, capacity=128, head_dim=128):
