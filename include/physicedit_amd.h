@@ -372,7 +372,7 @@ typedef struct pe_logits_args {
 int pe_process_logits(const pe_logits_args* a, float* out, void* stream);
 /* token[row] = first maximum of the processed scores (NaN is never chosen), -1 where all are -inf.  update_counts != 0: the token's count goes up by one
  * (it stays at 32767).  step (device, rows == 1 only, nullable): out_ids[*step] = token while *step < max_steps, then *step += 1 -- pe_decode_argmax's
- * convention.  workspace: pe_select_token_workspace_bytes bytes, private to the stream. */
+ * convention.  workspace: pe_select_token_workspace_bytes bytes (none for small vocabularies), private to the stream. */
 size_t pe_select_token_workspace_bytes(int rows, int vocab);
 int pe_select_token(const pe_logits_args* a, int* token, int update_counts, int* out_ids, int* step, int max_steps, void* workspace,
                     size_t workspace_bytes, void* stream);

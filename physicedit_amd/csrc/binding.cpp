@@ -312,12 +312,11 @@ PyObject* select_token(PyObject*, PyObject* const* a, Py_ssize_t n) {
         }
         at::Tensor out, ws;
         if (!to) { out = empty_like_type(x, {s.rows}, at::kInt); to = (int*)out.data_ptr(); }
-        void* wp;
-        size_t wn;
+        void* wp = nullptr;
+        size_t wn = 0;
         if (a[9] == Py_None) {
             wn = api.select_token_workspace_bytes(s.rows, s.vocab);
-            ws = empty_like_type(x, {(int64_t)wn}, at::kByte);
-            wp = ws.data_ptr();
+            if (wn) { ws = empty_like_type(x, {(int64_t)wn}, at::kByte); wp = ws.data_ptr(); }
         } else {
             const at::Tensor& t = tensor(a[9], "workspace");
             if (!on(t, (int)dev) || !t.is_contiguous()) bad("workspace: expected a contiguous tensor on cuda:%ld", dev);

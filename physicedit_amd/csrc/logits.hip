@@ -50,7 +50,7 @@ PE_DEV f32x8 process8(const LogitsArgs& a, size_t row, int v, float rep, float p
     const T* lg = (const T*)a.logits + row * a.ld + v;
     const short* ct = a.counts ? a.counts + row * a.ldc + v : nullptr;
     const float* bs = a.bias ? a.bias + row * a.ldb + v : nullptr;
-    const uint32_t bits = a.allowed ? a.allowed[row * a.ldm + (v >> 5)] >> (v & 31) : 0xffu;
+    const uint32_t word = a.allowed ? a.allowed[row * a.ldm + (v >> 5)] : 0xffffffffu;       // used last: a shift here would wait for it alone
     f32x8 x, b = {};
     s16x8 n = {};
     if (v + 8 <= a.V) {
@@ -66,6 +66,7 @@ PE_DEV f32x8 process8(const LogitsArgs& a, size_t row, int v, float rep, float p
             b[e] = in && bs ? bs[e] : 0.f;
         }
     }
+    const uint32_t bits = word >> (v & 31);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const bool ok = ((bits >> e) & 1) && v + e < a.V;
@@ -76,9 +77,13 @@ PE_DEV f32x8 process8(const LogitsArgs& a, size_t row, int v, float rep, float p
 }
 
 PE_DEV void row_penalties(const LogitsArgs& a, size_t row, float& rep, float& presence, float& frequency) {
-    rep = a.penalties ? a.penalties[row * a.ldp] : 1.f;
-    presence = a.penalties ? a.penalties[row * a.ldp + 1] : 0.f;
-    frequency = a.penalties ? a.penalties[row * a.ldp + 2] : 0.f;
+    // vector loads of a uniform address: a scalar load's wait is a wait for all of them, here it joins the queue of the scores
+    int zero;
+    asm("v_mov_b32 %0, 0" : "=v"(zero));
+    const float* p = a.penalties + row * a.ldp + zero;
+    rep = a.penalties ? p[0] : 1.f;
+    presence = a.penalties ? p[1] : 0.f;
+    frequency = a.penalties ? p[2] : 0.f;
 }
 
 template <typename T>
@@ -109,32 +114,6 @@ PE_DEV void wave_best(float& best, int& idx) {
     for (int o = 32; o > 0; o >>= 1) better(best, idx, __shfl_xor(best, o, 64), __shfl_xor(idx, o, 64));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) select_part_kernel(LogitsArgs a, float* part_v, int* part_i) {
-    __shared__ float bv[4];
-    __shared__ int bi[4];
-    const size_t row = blockIdx.y;
-    float rep, presence, frequency;
-    row_penalties(a, row, rep, presence, frequency);
-    float best = -INFINITY;
-    int idx = NONE;
-    const int v = (int)(blockIdx.x * 256 + threadIdx.x) * 8;
-    if (v < a.V) {
-        const f32x8 x = process8<T>(a, row, v, rep, presence, frequency);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (x[e] > best) { best = x[e]; idx = v + e; }
-    }
-    wave_best(best, idx);
-    if (lane_id() == 0) { bv[wave_id()] = best; bi[wave_id()] = idx; }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 4; ++w) better(best, idx, bv[w], bi[w]);
-        part_v[row * gridDim.x + blockIdx.x] = best;
-        part_i[row * gridDim.x + blockIdx.x] = idx;
-    }
-}
-
 // bits 0 .. 14 of a count go up by one and stop at 32767; two tokens share a 32-bit word.  Only the token's own half changes, so any
 // order of concurrent additions gives the same counts.
 PE_DEV void count_token(short* counts, int v, bool prompt) {
@@ -151,6 +130,51 @@ PE_DEV void count_token(short* counts, int v, bool prompt) {
     } while (old != seen);
 }
 
+// what becomes of a row's choice
+PE_DEV void take_token(int idx, size_t row, int* token, short* counts, long long ldc, int* out_ids, int* step, int max_steps) {
+    const int t = idx == NONE ? -1 : idx;
+    token[row] = t;
+    if (counts && t >= 0) count_token(counts + row * ldc, t, false);
+    if (step) {                                   // one row only: the decode step's counter
+        const int st = *step;
+        if (st >= 0 && st < max_steps) out_ids[st] = t;
+        *step = st + 1;
+    }
+}
+
+// A row's best in one work-group (up to 8192 tokens: one launch instead of two) or a part's.  THREADS lanes of 8 tokens.
+template <typename T, int THREADS, bool WHOLE>
+__global__ void __launch_bounds__(THREADS) select_part_kernel(LogitsArgs a, float* part_v, int* part_i, int* token, short* counts, int* out_ids, int* step,
+                                                              int max_steps) {
+    __shared__ float bv[THREADS / 64];
+    __shared__ int bi[THREADS / 64];
+    const size_t row = blockIdx.y;
+    float rep, presence, frequency;
+    row_penalties(a, row, rep, presence, frequency);
+    float best = -INFINITY;
+    int idx = NONE;
+#pragma unroll 2
+    for (int v = (int)(blockIdx.x * THREADS + threadIdx.x) * 8; v < a.V; v += THREADS * 8) {
+        const f32x8 x = process8<T>(a, row, v, rep, presence, frequency);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (x[e] > best) { best = x[e]; idx = v + e; }        // ascending: the first maximum stays
+        if (!WHOLE) break;
+    }
+    wave_best(best, idx);
+    if (lane_id() == 0) { bv[wave_id()] = best; bi[wave_id()] = idx; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < THREADS / 64; ++w) better(best, idx, bv[w], bi[w]);
+        if (WHOLE) {
+            take_token(idx, row, token, counts, a.ldc, out_ids, step, max_steps);
+        } else {
+            part_v[row * gridDim.x + blockIdx.x] = best;
+            part_i[row * gridDim.x + blockIdx.x] = idx;
+        }
+    }
+}
+
 __global__ void __launch_bounds__(64) select_join_kernel(const float* part_v, const int* part_i, int parts, int* token, short* counts,
                                                          long long ldc, int* out_ids, int* step, int max_steps) {
     const size_t row = blockIdx.x;
@@ -158,16 +182,7 @@ __global__ void __launch_bounds__(64) select_join_kernel(const float* part_v, co
     int idx = NONE;
     for (int i = lane_id(); i < parts; i += 64) better(best, idx, part_v[row * parts + i], part_i[row * parts + i]);
     wave_best(best, idx);
-    if (lane_id() == 0) {
-        const int t = idx == NONE ? -1 : idx;
-        token[row] = t;
-        if (counts && t >= 0) count_token(counts + row * ldc, t, false);
-        if (step) {                               // one row only: the decode step's counter
-            const int st = *step;
-            if (st >= 0 && st < max_steps) out_ids[st] = t;
-            *step = st + 1;
-        }
-    }
+    if (lane_id() == 0) take_token(idx, row, token, counts, ldc, out_ids, step, max_steps);
 }
 
 __global__ void __launch_bounds__(256) token_counts_add_kernel(short* counts, long long ldc, int V, const int* tokens, int n, int prompt) {
@@ -200,8 +215,11 @@ int launch_process_logits(const LogitsArgs& a, hipStream_t stream) {
     return check_launch("process_logits_kernel");
 }
 
+// one work-group reads a short row in the time that a second launch costs (1 row, bf16 with counts: 2000 tokens 3.6 us against 5.4, 8000 5.1 and 5.8,
+// 16000 7.1 and 5.9)
+constexpr int SELECT_WHOLE = 8192;
 size_t select_token_workspace_bytes(int rows, int V) {
-    return rows < 1 || V < 1 ? 0 : (size_t)rows * ((V + LOGITS_PER_BLOCK - 1) / LOGITS_PER_BLOCK) * 8;
+    return rows < 1 || V <= SELECT_WHOLE ? 0 : (size_t)rows * ((V + LOGITS_PER_BLOCK - 1) / LOGITS_PER_BLOCK) * 8;
 }
 
 int launch_select_token(const LogitsArgs& a, int* token, short* count_into, int* out_ids, int* step, int max_steps, void* workspace,
@@ -210,12 +228,20 @@ int launch_select_token(const LogitsArgs& a, int* token, short* count_into, int*
     PE_REQUIRE(token, "select_token: null token");
     PE_REQUIRE(!step || (out_ids && max_steps >= 1 && a.rows == 1), "select_token: a step counter belongs to one row and its list of tokens");
     const size_t need = select_token_workspace_bytes(a.rows, a.V);
-    PE_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 3) == 0, "select_token: workspace of %zu bytes needed", need);
+    PE_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 3) == 0), "select_token: workspace of %zu bytes needed", need);
     const int parts = (a.V + LOGITS_PER_BLOCK - 1) / LOGITS_PER_BLOCK;
     float* pv = (float*)workspace;
     int* pi = (int*)(pv + (size_t)a.rows * parts);
-    if (a.f32) hipLaunchKernelGGL(select_part_kernel<float>, dim3(parts, a.rows), dim3(256), 0, stream, a, pv, pi);
-    else hipLaunchKernelGGL(select_part_kernel<bf16>, dim3(parts, a.rows), dim3(256), 0, stream, a, pv, pi);
+#define PE_SELECT(T, THREADS, WHOLE, X)                                                                                          \
+    hipLaunchKernelGGL((select_part_kernel<T, THREADS, WHOLE>), dim3(X, a.rows), dim3(THREADS), 0, stream, a, pv, pi, token, count_into, out_ids, step, max_steps)
+    if (need == 0) {
+        if (a.V <= LOGITS_PER_BLOCK) { if (a.f32) PE_SELECT(float, 256, true, 1); else PE_SELECT(bf16, 256, true, 1); }
+        else { if (a.f32) PE_SELECT(float, 1024, true, 1); else PE_SELECT(bf16, 1024, true, 1); }
+        return check_launch("select_part_kernel");
+    }
+    if (a.f32) PE_SELECT(float, 256, false, parts);
+    else PE_SELECT(bf16, 256, false, parts);
+#undef PE_SELECT
     if (const int rc = check_launch("select_part_kernel")) return rc;
     hipLaunchKernelGGL(select_join_kernel, dim3(a.rows), dim3(64), 0, stream, pv, pi, parts, token, count_into, a.ldc, out_ids, step, max_steps);
     return check_launch("select_join_kernel");

@@ -212,7 +212,7 @@ int launch_gemv_w4(const W4Problem& p, hipStream_t stream) {
     a.eps = p.eps;
     const int gs = p.group / 32;
     // Weight tiles (R) and waves (W) of a work-group.  At most a tile per CU: each gets all the waves that fit (N = 3584, K = 18944, one row: R, W = 1, 16
-    // 12.3 us, 1, 8 17.2, 2, 8 20.7).  Some per CU: R = 1 leaves them balanced (N = 10000, K = 3584: 1, 8 7.0 us, 4, 8 8.8).  Many: a work-group's start,
+    // 12.3 us, 1, 8 17.2, 2, 8 20.7); up to two, the same with pairs (N = 5120, K = 13824: 2, 16 12.1 us, 1, 8 14.9, 1, 16 16.1).  Some per CU: R = 1 leaves them balanced (N = 10000, K = 3584: 1, 8 7.0 us, 4, 8 8.8).  Many: a work-group's start,
     // end and reads of x are shared (N = 152064: 1, 8 79.5 us, 2, 8 65.9, 4, 8 53.2).  From two row tiles on x weighs more (20 rows, N = 5001: 1, 8 11.1 us, 2, 8 10.1;
     // 33: 19.1 and 13.1), from three on its chunks fill the LDS (60 rows, N = 12001: 2, 8 18.1 us, 2, 4 15.0, 4, 4 17.3; 64 rows, N = 152064: 199, 179, 202).
     const int tiles = (p.N + 15) / 16, mt = (p.M + 15) / 16;
@@ -220,6 +220,7 @@ int launch_gemv_w4(const W4Problem& p, hipStream_t stream) {
     // The gated epilogue works on pairs of tiles: with many, one pair and four waves for few rows (N = 37888, one row: 2, 4 18.4 us, 4, 8 19.7; 16 rows: 22.0, 21.3).
 #define PE_W4(MT, R, W) { if (p.swiglu) w4_launch<MT, (R == 1 ? 2 : R), (R == 1 ? 8 : W), true>(a, gs, p.norm, stream); else w4_launch<MT, R, W, false>(a, gs, p.norm, stream); }
     if (p.swiglu && size == 2 && p.M <= 8) w4_launch<1, 2, 4, true>(a, gs, p.norm, stream);
+    else if (!p.swiglu && mt == 1 && size == 1 && tiles <= 512) w4_launch<1, 2, 16, false>(a, gs, p.norm, stream);
     else
     if (mt == 1) { if (size == 0) PE_W4(1, 1, 16) else if (size == 1) PE_W4(1, 1, 8) else PE_W4(1, 4, 8) }
     else if (mt == 2) { if (size == 0) PE_W4(2, 1, 8) else if (size == 1) PE_W4(2, 2, 8) else PE_W4(2, 4, 8) }

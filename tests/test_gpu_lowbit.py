@@ -600,7 +600,7 @@ def scores_case(g, R, V, dtype):
     return logits, counts, torch.tensor([1.3, 0.4, 0.01], device="cuda") * (1 + 0.1 * torch.rand((R, 3), generator=g, device="cuda")), randn(g, R, V), allowed
 
 
-@pytest.mark.parametrize("R,V", [(1, 1), (1, 7), (2, 8), (3, 33), (1, 2048), (2, 2049), (5, 4097), (1, 152064), (9, 50001)])
+@pytest.mark.parametrize("R,V", [(1, 1), (1, 7), (2, 8), (3, 33), (1, 2048), (2, 2049), (5, 4097), (3, 8192), (1, 8193), (2, 16385), (1, 152064), (9, 50001)])
 @pytest.mark.parametrize("dtype", [BF, torch.float32])
 def test_process_and_select(ops, R, V, dtype):
     g = gen(V)
@@ -706,4 +706,4 @@ def test_logits_refusals(ops):
             bad()
     from physicedit_amd._lib import PeError
     with pytest.raises(PeError, match="workspace"):
-        ops.select_token(x, workspace=torch.empty((8,), dtype=torch.uint8, device="cuda"))
+        ops.select_token(torch.zeros((2, 50000), device="cuda"), workspace=torch.empty((8,), dtype=torch.uint8, device="cuda"))

@@ -104,6 +104,7 @@ def test_workspace_sizes(lib):
     assert lib.pe_kv_attention_workspace_bytes(1, 4, 1, 28, 128, 15360) >= 2 * 28 * 130 * 4
     assert lib.pe_kv_attention_workspace_bytes(0, 4, 1, 28, 128, 15360) == 0
     assert lib.pe_select_token_workspace_bytes(3, 152064) == 3 * 75 * 8 and lib.pe_select_token_workspace_bytes(0, 5) == 0
+    assert lib.pe_select_token_workspace_bytes(3, 8192) == 0 and lib.pe_select_token_workspace_bytes(1, 8193) == 5 * 8
 
 
 @pytest.mark.parametrize("args,text", [
@@ -124,7 +125,8 @@ def test_select_and_counts_refusals(lib):
     refused(lib, lib.pe_select_token(C.byref(s), None, 0, None, None, 0, P, 1 << 20, None), "null token")
     refused(lib, lib.pe_select_token(C.byref(s), P, 1, None, None, 0, P, 1 << 20, None), "no counts")
     refused(lib, lib.pe_select_token(C.byref(s), P, 0, P, P, 8, P, 1 << 20, None), "one row")
-    refused(lib, lib.pe_select_token(C.byref(s), P, 0, None, None, 0, P, 8, None), "workspace of 16")
+    big = L.LogitsArgs(logits=P, ld=100000, rows=2, vocab=100000)
+    refused(lib, lib.pe_select_token(C.byref(big), P, 0, None, None, 0, P, 8, None), "workspace of 784")
     refused(lib, lib.pe_token_counts_add(None, 100, 2, 100, P, 3, 0, None), "null")
     refused(lib, lib.pe_token_counts_add(P, 99, 2, 100, P, 3, 0, None), "bad shape")
     refused(lib, lib.pe_token_counts_add(P, 100, 2, 100, P, 0, 0, None), "bad shape")
