@@ -519,11 +519,27 @@ def _at(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, shape, dev: in
     return t.data_ptr()
 
 
-class W4Weight:
+class _Held:
+    """attributes that are set once: the struct made from them holds their addresses"""
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__:
+            raise AttributeError(f"{type(self).__name__}.{name} cannot be replaced: the kernels hold its address (copy_ into it, or make a new one)")
+        super().__setattr__(name, value)
+
+
+class W4Weight(_Held):
     """A linear's weight [N, K] as 4-bit codes with a scale (and a zero point) per output and `group` inputs, in the layout of pe_gemv_w4
-    (include/physicedit_amd.h, pe_w4_weight).  Made by pack_w4 / quantize_w4."""
+    (include/physicedit_amd.h, pe_w4_weight): codes uint8 [ceil(N/16), ceil(K/128), 64, 16], scale bf16 [ceil(N/16), groups, 16, 2].  Made by
+    pack_w4 / quantize_w4."""
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor, N: int, K: int, group: int):
+        tiles, chunks = (N + 15) // 16, (K + 127) // 128
+        if (group not in (32, 64, 128) or N < 1 or K < group or K % group or codes.dtype is not torch.uint8 or codes.shape != (tiles, chunks, 64, 16)
+                or scale.dtype is not BF or scale.shape != (tiles, chunks * (128 // group), 16, 2) or codes.device != scale.device
+                or not codes.is_contiguous() or not scale.is_contiguous()):
+            raise ValueError(f"W4Weight: N={N} K={K} group={group} with codes {codes.dtype} {tuple(codes.shape)} and scale {scale.dtype} {tuple(scale.shape)} "
+                             f"(contiguous uint8 [ceil(N/16), ceil(K/128), 64, 16] and bf16 [ceil(N/16), groups, 16, 2] on one device)")
         self.codes, self.scale, self.N, self.K, self.group = codes, scale, N, K, group
         self._c = _lib.W4Weight(codes.data_ptr(), scale.data_ptr(), N, K, group)
         self._addr, self._dev = C.addressof(self._c), codes.get_device()
@@ -603,7 +619,7 @@ def gemv_w4(x: torch.Tensor, w: W4Weight, bias: Optional[torch.Tensor] = None, r
     return _binding().gemv_w4(x, w._addr, w._dev, bias, res, epilogue == "swiglu", -1.0 if norm_eps is None else norm_eps, out)
 
 
-class KVCacheE4M3:
+class KVCacheE4M3(_Held):
     """The keys and values of one layer as e4m3 codes with a scale per (sequence, token, kv head), zero at first.  capacity: a multiple of 64.
     Views of the buffers: k [batch, n_kv, capacity, head_dim], v [batch, n_kv, capacity/64, 64, head_dim] (stored transposed in blocks of
     64 tokens), k_scale / v_scale [batch, n_kv, capacity]; value = code * scale."""

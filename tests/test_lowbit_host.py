@@ -169,3 +169,21 @@ def test_pack_w4_layout(monkeypatch, N, K, group):
         assert torch.equal(pair[:N, :K // group, 1].float(), -128.0 - (zero.float() if z is not None else torch.full((N, K // group), 8.0)))
         assert not pair[N:].any() and not pair[:, K // group:].any()
         assert w.nbytes == tiles * chunks * 1024 + pair.numel() * 2
+
+
+def test_weights_and_caches_hold_their_buffers():
+    """the structs passed to the kernels hold addresses: parts of another shape are refused, and the buffers behind the addresses cannot be exchanged"""
+    from physicedit_amd import ops
+    codes, scale = torch.zeros((3, 2, 64, 16), dtype=torch.uint8), torch.zeros((3, 8, 16, 2), dtype=BF)
+    w = ops.W4Weight(codes, scale, 33, 256, 32)
+    assert w.codes is codes and w.scale is scale
+    for args in ((codes[:2], scale, 33, 256, 32), (codes, scale[:2], 33, 256, 32), (codes, scale, 49, 256, 32), (codes, scale, 33, 260, 32), (codes, scale, 33, 288, 32),
+                 (codes, scale, 33, 256, 64), (codes, scale, 33, 256, 16), (codes.char(), scale, 33, 256, 32), (codes, scale.half(), 33, 256, 32),
+                 (codes.transpose(0, 1).contiguous().transpose(0, 1), scale, 33, 256, 32), (codes, scale.to("meta"), 33, 256, 32), (codes, scale, 0, 256, 32)):
+        with pytest.raises(ValueError, match="W4Weight"):
+            ops.W4Weight(*args)
+    cache = ops.KVCacheE4M3(1, 2, 64, 64, device="cpu")
+    for obj, names in ((w, ("codes", "scale", "N", "K", "group")), (cache, ("k", "v", "k_scale", "v_scale", "batch", "n_kv", "capacity", "head_dim"))):
+        for name in names:
+            with pytest.raises(AttributeError):
+                setattr(obj, name, getattr(obj, name))
