@@ -93,6 +93,18 @@ void* heads_(const at::Tensor& t, const char* name, at::IntArrayRef shape, long 
     return p;
 }
 
+// A result that the caller passed lies apart from input `in` -- or, where `over` says that each of its elements is read before it is written, exactly over it.
+// A dimension of strides counts with all that lies between its ends.
+void apart(PyObject* result, PyObject* in, const char* name, bool over = false) {
+    if (result == Py_None || in == Py_None) return;
+    const at::Tensor &r = tensor(result, "out"), &t = tensor(in, name);
+    int64_t span = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) span += (t.size(i) - 1) * t.stride(i);
+    const char *r0 = (const char*)r.data_ptr(), *t0 = (const char*)t.data_ptr(), *r1 = r0 + r.nbytes(), *t1 = t0 + span * (int64_t)t.element_size();
+    if (r1 <= t0 || t1 <= r0 || (over && r0 == t0 && t.is_contiguous() && t.nbytes() == r.nbytes())) return;
+    bad("out: overlaps %s%s", name, over ? " (it may only lie exactly over it)" : "");
+}
+
 const at::Tensor& four_dims(PyObject* o, const char* name, const char* what) {
     const at::Tensor& t = tensor(o, name);
     if (t.dim() != 4) bad("%s: expected %s, got %s", name, what, show(t).c_str());
@@ -162,6 +174,9 @@ PyObject* gemv_w4(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const void *bias = at_(a[3], "bias", at::kBFloat16, {(int64_t)w->N}, dev), *res = at_(a[4], "res", at::kBFloat16, shape, dev);
         void* to = at_(a[7], "out", at::kBFloat16, shape, dev);
         if (M < 1 || M > 1 << 20) bad("gemv_w4: %lld rows", (long long)M);
+        apart(a[7], a[3], "bias");
+        apart(a[7], a[4], "res", true);
+        if (to != x.data_ptr()) apart(a[7], a[0], "x");        // at x itself: the library's own refusal
         at::Tensor out;
         if (a[7] == Py_None) { out = empty_like_type(x, shape, at::kBFloat16); to = out.data_ptr(); }
         const float eps = (float)number(a[6]);
@@ -206,6 +221,11 @@ PyObject* kv_append_e4m3(PyObject*, PyObject* const* a, Py_ssize_t n) {
             s.q = heads_(q, "q", {B, T, nq, D}, dev, s.q_strides);
             s.q_out = at_(a[9], "out", at::kBFloat16, {B, T, nq, D}, dev);
             if (a[9] == Py_None) { out = empty_like_type(q, {B, T, nq, D}, at::kBFloat16); s.q_out = out.data_ptr(); }
+            apart(a[9], a[5], "q", true);
+            apart(a[9], a[2], "k");
+            apart(a[9], a[3], "v");
+            apart(a[9], a[6], "cos");
+            apart(a[9], a[7], "sin");
         }
         launch("pe_kv_append_e4m3", [&] { return api.kv_append_e4m3(c, &s, stream); });
         if (!has_q) Py_RETURN_NONE;
@@ -230,6 +250,8 @@ PyObject* kv_attention_e4m3(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const void* tree = at_(a[4], "tree", at::kLong, {B, T}, dev);
         const float scale = a[5] == Py_None ? (float)(1.0 / std::sqrt((double)D)) : (float)number(a[5]);
         void* to = at_(a[6], "out", at::kBFloat16, {B, T, nq * D}, dev);
+        apart(a[6], a[0], "q", true);
+        apart(a[6], a[7], "workspace");
         at::Tensor out, ws;
         if (a[6] == Py_None) { out = empty_like_type(q, {B, T, nq * D}, at::kBFloat16); to = out.data_ptr(); }
         void* wp = nullptr;
@@ -285,6 +307,11 @@ PyObject* process_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
         void* to = at_(a[5], "out", at::kFloat, {s.rows, s.vocab}, dev);
         at::Tensor out;
         if (a[5] == Py_None) { out = empty_like_type(tensor(a[0], "logits"), {s.rows, s.vocab}, at::kFloat); to = out.data_ptr(); }
+        apart(a[5], a[0], "logits", true);
+        apart(a[5], a[1], "counts");
+        apart(a[5], a[2], "penalties");
+        apart(a[5], a[3], "bias", true);
+        apart(a[5], a[4], "allowed");
         launch("pe_process_logits", [&] { return api.process_logits(&s, (float*)to, stream); });
         return wrap_or(a[5], out);
     });
@@ -310,6 +337,15 @@ PyObject* select_token(PyObject*, PyObject* const* a, Py_ssize_t n) {
             ids = (int*)at_(a[7], "out_ids", at::kInt, {room}, dev);
             step = (int*)at_(a[8], "step", at::kInt, tensor(a[8], "step").sizes(), dev);
         }
+        for (int i = 0; i < 5; ++i) {
+            static const char* const names[5] = {"logits", "counts", "penalties", "bias", "allowed"};
+            apart(a[6], a[i], names[i]);
+            apart(a[7], a[i], names[i]);
+            apart(a[8], a[i], names[i]);
+        }
+        apart(a[6], a[7], "out_ids");
+        apart(a[6], a[8], "step");
+        apart(a[7], a[8], "step");
         at::Tensor out, ws;
         if (!to) { out = empty_like_type(x, {s.rows}, at::kInt); to = (int*)out.data_ptr(); }
         void* wp = nullptr;

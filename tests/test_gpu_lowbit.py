@@ -707,3 +707,54 @@ def test_logits_refusals(ops):
     from physicedit_amd._lib import PeError
     with pytest.raises(PeError, match="workspace"):
         ops.select_token(torch.zeros((2, 50000), device="cuda"), workspace=torch.empty((8,), dtype=torch.uint8, device="cuda"))
+
+
+def test_results_over_their_inputs(ops):
+    """exactly over an input where the documentation allows it; any other overlap is refused, whichever side begins first"""
+    g = gen(12)
+    codes, scale, z, _ = w4_case(g, 1, 96, 128, 64, True)
+    w = ops.pack_w4(codes, scale, z, 64)
+    flat = randn(g, 4096).to(BF)
+    x, before = flat[1024:1024 + 256].view(2, 128), flat.clone()
+    for lo in (1024 - 64, 1024 + 64, 1024 + 128):                      # out [2, 96] across x's start, inside it, across its end
+        with pytest.raises(ValueError, match="overlaps x"):
+            ops.gemv_w4(x, w, out=flat[lo:lo + 192].view(2, 96))
+    with pytest.raises(ValueError, match="overlaps res"):
+        ops.gemv_w4(x, w, res=flat[2048:2240].view(2, 96), out=flat[2049:2241].view(2, 96))
+    with pytest.raises(ValueError, match="overlaps bias"):
+        ops.gemv_w4(x, w, bias=flat[2048:2144], out=flat[2048:2240].view(2, 96))
+    assert torch.equal(ops.gemv_w4(x, w, out=flat[1280:1472].view(2, 96)), ops.gemv_w4(x, w)) and torch.equal(flat[:1280], before[:1280]) and torch.equal(flat[1472:], before[1472:])
+
+    cache, twin = ops.KVCacheE4M3(2, 2, 512, 64), ops.KVCacheE4M3(2, 2, 512, 64)
+    start = torch.tensor([5, 300], dtype=torch.int32, device="cuda")
+    cos, sin = tables(512, 64, BF)
+    for T, hq in ((1, 6), (3, 6), (9, 6), (40, 2), (64, 10)):          # one, two, four row tiles of the attention and more
+        q, k, v = randn(g, 2, T, hq, 64).to(BF), randn(g, 2, T, 2, 64).to(BF), randn(g, 2, T, 2, 64).to(BF)
+        want = ops.kv_append_e4m3(twin, k, v, start, q=q, cos=cos, sin=sin)
+        with pytest.raises(ValueError, match="overlaps k"):
+            ops.kv_append_e4m3(cache, k, v, start, q=q[:, :, :2], cos=cos, sin=sin, out=k)
+        got = ops.kv_append_e4m3(cache, k, v, start, q=q, cos=cos, sin=sin, out=q)
+        assert got is q and torch.equal(q, want)
+        small, zero = ops.KVCacheE4M3(2, 2, 64, 64), torch.zeros_like(start)
+        ops.kv_append_e4m3(small, k, v, zero)
+        for c, s in ((cache, start), (small, zero)):                   # a cache walked in parts and one of one block
+            y = ops.kv_attention_e4m3(want, c, s)
+            over = want.clone()
+            assert torch.equal(ops.kv_attention_e4m3(over, c, s, out=over.view(2, T, -1)), y) and torch.equal(over.view(2, T, -1), y)
+        with pytest.raises(ValueError, match="overlaps q"):
+            ops.kv_attention_e4m3(want[:1].expand(2, T, hq, 64), cache, start, out=want.view(2, T, -1))
+
+    x = randn(g, 3, 1000)
+    counts, pen, bias, allowed = scores_case(g, 3, 1000, torch.float32)[1:]
+    want = ops.process_logits(x, counts, pen, bias, allowed)
+    over = x.clone()
+    assert torch.equal(ops.process_logits(over, counts, pen, bias, allowed, out=over), want) and torch.equal(over, want)
+    room = torch.zeros((3001,), device="cuda")
+    with pytest.raises(ValueError, match="overlaps logits"):
+        ops.process_logits(room[:3000].view(3, 1000), out=room[1:].view(3, 1000))
+    with pytest.raises(ValueError, match="overlaps bias"):
+        ops.process_logits(x, bias=room[:1000], out=room[:3000].view(3, 1000))
+    ids = torch.zeros((8,), dtype=torch.int32, device="cuda")
+    for out, out_ids, step in ((ids[:1], ids[:4], ids[5:6]), (ids[5:6], ids[:4], ids[5:6]), (ids[6:7], ids[:4], ids[3:4])):
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.select_token(x[:1], out=out, out_ids=out_ids, step=step)
