@@ -336,7 +336,7 @@ class GraphDecoder:
     a layer as one more matrix), weights="w4" also runs every linear of the step on 4-bit weights with a scale and zero point per output and
     `w4_group` inputs (pe_gemv_w4: a quarter of the weight bytes; q / k / v and gate / up are one matrix each, the RMSNorm weights folded into
     their columns).  The copies are made at the first call from the model's weights and again when those move or change (call reset() after
-    changing them through `.data`).
+    changing them through `.data`, or weights made under inference_mode: nothing counts those changes).
     Penalties and masks: a repetition_penalty or suppress_tokens of the generation config, or generate(prefix_allowed_tokens_fn=), make the
     next token the first maximum of the processed scores (pe_select_token) instead of the plain arg-max."""
 

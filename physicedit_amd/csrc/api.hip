@@ -337,6 +337,7 @@ int pe_decode_layer(const pe_decode_layer_weights* w, const void* x, void* x_out
 int pe_gemv_w4(const void* x, long long ldx, int M, const pe_w4_weight* w, const void* bias, const void* res, long long ldr, void* out,
                long long ldo, int swiglu, float norm_eps, void* stream) {
     PE_REQUIRE(w, "pe_gemv_w4: null weight");
+    PE_REQUIRE(norm_eps == norm_eps, "pe_gemv_w4: norm_eps is NaN");
     W4Problem p;
     p.x = x; p.ldx = ldx; p.M = M; p.N = w->N; p.K = w->K; p.group = w->group;
     p.codes = w->codes; p.scale = w->scale;

@@ -20,7 +20,8 @@
 // as a bf16, exact, above it: each is one instruction away from the fp32 it is used as.  N and K are padded to 16 and 128 with scales of 0.
 //
 // A work-group of W waves takes R tiles of 16 outputs; its waves take turns at the 128-input chunks and join their fp32 sums in LDS in a
-// fixed order: results do not depend on scheduling.  Lanes of rows >= M read row M - 1 again: their columns are never stored.
+// fixed order: results do not depend on scheduling.  Rows from M to the next multiple of four are row M - 1 again, those behind what the LDS held:
+// a row of x is a column of its own in every product, and theirs are never stored.
 #include "common.h"
 #include "kernels.h"
 
@@ -202,7 +203,6 @@ int launch_gemv_w4(const W4Problem& p, hipStream_t stream) {
     PE_REQUIRE(!(p.swiglu && p.res), "gemv_w4: no residual with the gated epilogue");
     PE_REQUIRE(p.out != p.x, "gemv_w4: out may be res, not x (every work-group reads all of x)");
     PE_REQUIRE(p.ldo >= cols && (!p.res || p.ldr >= cols), "gemv_w4: row stride below the %d columns", cols);
-    PE_REQUIRE(!p.norm || p.eps >= 0.f, "gemv_w4: negative eps");
     W4Args a;
     a.x = (const bf16*)p.x; a.codes = (const u32x4*)p.codes; a.scale = (const u32x4*)p.scale;
     a.bias = (const bf16*)p.bias; a.res = (const bf16*)p.res; a.out = (bf16*)p.out;

@@ -187,3 +187,8 @@ def test_weights_and_caches_hold_their_buffers():
         for name in names:
             with pytest.raises(AttributeError):
                 setattr(obj, name, getattr(obj, name))
+
+
+def test_gemv_w4_eps_is_a_number(lib):
+    """a NaN is not "no norm" """
+    refused(lib, lib.pe_gemv_w4(P, 256, 1, C.byref(w4()), None, None, 32, 2 * P, 32, 0, float("nan"), None), "norm_eps")
