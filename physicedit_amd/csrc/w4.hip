@@ -91,6 +91,10 @@ __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
 #pragma unroll
             for (int g = 0; g < GC; ++g) sc[r][g] = a.scale[((size_t)tile[r] * a.G + kc * GC + g) * 4 + j];
         __builtin_amdgcn_sched_barrier(0);      // or the scheduler sinks the loads to their uses to save registers, one round trip after another
+        // x is in LDS when at most the R (1 + GC) younger loads are under way.  (The compiler's own wait for copies into LDS is not there in every variant.)
+        constexpr int YOUNGER = R * (1 + GC);
+        __builtin_amdgcn_s_waitcnt((YOUNGER & 15) | (YOUNGER >> 4) << 14 | 0x0f70);      // vmcnt(YOUNGER) alone
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll

@@ -124,6 +124,20 @@ def test_gemv_w4(ops, M, N, K, group, zero, norm, bias, res, swiglu):
     near(got, want, slack)
 
 
+@pytest.mark.parametrize("M", [1, 8, 16, 20, 33, 60])
+@pytest.mark.parametrize("N", [1888, 8096, 12064, 17504])          # 118, 506, 754, 1094 tiles of 16: each side of the rules on their number
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_gemv_w4_variants(ops, M, N, group):
+    """every kernel that the rules on sizes choose, with more chunks of 128 inputs than waves and the last one cut short"""
+    g = gen(M * N + group)
+    codes, scale, z, x = w4_case(g, M, N, 128 * 34 + group, group, True)
+    w, plain = ops.pack_w4(codes, scale, z, group), w4_weight(codes, scale, z, group)
+    for norm in (False, True):
+        for swiglu in (False, True):
+            got = ops.gemv_w4(x, w, epilogue="swiglu" if swiglu else "bias", norm_eps=1e-6 if norm else None)
+            near(got, *w4_reference(plain, scale, group, x, 1e-6 if norm else None, None, None, swiglu))
+
+
 def test_gemv_w4_forms_of_the_call(ops):
     """one row as a vector, rows with a stride, the residual overwritten in place, another stream, rows that do not touch one another"""
     g = gen(3)
