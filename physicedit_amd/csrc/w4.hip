@@ -70,27 +70,35 @@ __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) ones[e] = (bf16)1.0f;
 
+    // A chunk on its way.  x goes straight into LDS, four rows of 256 bytes an instruction: 16 consecutive lanes read one row.  (As fragments, 16 lanes read
+    // 16 rows and a load takes 64 steps of the address unit instead of 16: N = 3584, K = 18944, 7 rows 18.6 us against 13.9, 64 rows 74.6 against 38.0.)
+    // Piece p (16 bytes) of row m goes to slot p ^ (m & 15): the fragment reads below find their 16 rows in 16 different slots.  The steps that pad K have
+    // scales of 0 (their groups are padding too), their x is any part of the row.  The barriers: or the scheduler sinks the loads to their uses to save
+    // registers, one round trip after another.
+#define PE_W4_FETCH(CHUNK, WQ, SC)                                                                                                      \
+    {                                                                                                                                   \
+        _Pragma("unroll") for (int q = 0; q < MT * 4; ++q)                                                                              \
+            if (4 * q < a.M) {                                                                                                          \
+                const int m = 4 * q + j, k = (CHUNK) * 128 + 8 * (c ^ (m & 15));                                                        \
+                glds16(a.x + (size_t)min(m, a.M - 1) * a.ldx + min(k, a.K - 8), stage[w] + q * 1024);                                   \
+            }                                                                                                                           \
+        __builtin_amdgcn_sched_barrier(0);                                                                                              \
+        _Pragma("unroll") for (int r = 0; r < R; ++r)                                                                                   \
+            WQ[r] = __builtin_nontemporal_load(a.codes + ((size_t)tile[r] * a.KC + (CHUNK)) * 64 + lane);                               \
+        _Pragma("unroll") for (int r = 0; r < R; ++r)                                                                                   \
+            _Pragma("unroll") for (int g = 0; g < GC; ++g) SC[r][g] = a.scale[((size_t)tile[r] * a.G + (CHUNK) * GC + g) * 4 + j];      \
+        __builtin_amdgcn_sched_barrier(0);                                                                                              \
+    }
+    // Waves that take many chunks of few tiles ask for the next chunk as soon as this one is in registers (N = 3584, K = 18944: one row 13.5 -> 12.4 us, 24
+    // rows 22.6 -> 20.2; 33 rows, N = 37888, gated: 46.9 -> 40.6).  Elsewhere the registers cost more waves than that hides (N = 152064, one row: R = 4
+    // 55.5 -> 72; 60 rows, N = 12001, R, W = 2, 4: 15.3 -> 21.3).
+    constexpr bool AHEAD = R == 1 || (MT == 3 && W == 4);
+    u32x4 nq[R], ns[R][GC];
+    if (AHEAD && w < a.KC) PE_W4_FETCH(w, nq, ns)
     for (int kc = w; kc < a.KC; kc += W) {
         u32x4 wq[R], sc[R][GC];
         bf16x8 b[MT][4];
-        // x straight into LDS, four rows of 256 bytes an instruction: 16 consecutive lanes read one row.  (As fragments, 16 lanes read 16 rows and a load
-        // takes 64 steps of the address unit instead of 16: N = 3584, K = 18944, 7 rows 18.6 us against 13.9, 64 rows 74.6 against 38.0.)  Piece p
-        // (16 bytes) of row m goes to slot p ^ (m & 15): the fragment reads below find their 16 rows in 16 different slots.  The steps that pad K have
-        // scales of 0 (their groups are padding too), their x is any part of the row.
-#pragma unroll
-        for (int q = 0; q < MT * 4; ++q)
-            if (4 * q < a.M) {
-                const int m = 4 * q + j, k = kc * 128 + 8 * (c ^ (m & 15));
-                glds16(a.x + (size_t)min(m, a.M - 1) * a.ldx + min(k, a.K - 8), stage[w] + q * 1024);
-            }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int r = 0; r < R; ++r) wq[r] = __builtin_nontemporal_load(a.codes + ((size_t)tile[r] * a.KC + kc) * 64 + lane);
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int g = 0; g < GC; ++g) sc[r][g] = a.scale[((size_t)tile[r] * a.G + kc * GC + g) * 4 + j];
-        __builtin_amdgcn_sched_barrier(0);      // or the scheduler sinks the loads to their uses to save registers, one round trip after another
+        if (!AHEAD) PE_W4_FETCH(kc, wq, sc)
         // x is in LDS when at most the R (1 + GC) younger loads are under way.  (The compiler's own wait for copies into LDS is not there in every variant.)
         constexpr int YOUNGER = R * (1 + GC);
         __builtin_amdgcn_s_waitcnt((YOUNGER & 15) | (YOUNGER >> 4) << 14 | 0x0f70);      // vmcnt(YOUNGER) alone
@@ -99,6 +107,18 @@ __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
         for (int s = 0; s < 4; ++s)
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) b[mt][s] = *(const bf16x8*)(stage[w] + (mt * 16 + c) * 256 + ((4 * s + j) ^ c) * 16);
+        if (AHEAD) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                wq[r] = nq[r];
+#pragma unroll
+                for (int g = 0; g < GC; ++g) sc[r][g] = ns[r][g];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(0x0070);         // vmcnt(0) lgkmcnt(0): the chunk is in registers, its place in LDS is free
+            __builtin_amdgcn_sched_barrier(0);
+            if (kc + W < a.KC) PE_W4_FETCH(kc + W, nq, ns)
+        }
         if (NORM) {
 #pragma unroll
             for (int s = 0; s < 4; ++s)
@@ -133,6 +153,7 @@ __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
                 }
         }
     }
+#undef PE_W4_FETCH
 
     if (NORM) {             // the diagonal: row 4 j + i == column c
 #pragma unroll
