@@ -247,6 +247,13 @@ PE_DEV float sum_over_j(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// rows of the cache that exist, and how many of the splits have a block of them (the first always takes part)
+PE_DEV int kv_rows(int start, int T, int cap) { return start < 0 ? 0 : min(min(start, cap) + T, cap); }
+PE_DEV int kv_used_splits(int start, int T, int cap, int splits) {
+    const int blocks = (kv_rows(start, T, cap) + 63) >> 6, per = (blocks + splits - 1) / splits;
+    return per == 0 ? 1 : (blocks + per - 1) / per;
+}
+
 // WR row tiles x WK shares of the cache's blocks = the waves of a work-group: with one row tile (decode: T * n_q / H <= 16 rows) all waves share its
 // blocks and are joined in LDS; with more rows a wave takes 16 of them and the waves read the same blocks through the cache.
 template <int D, int WR, int WK>
@@ -262,10 +269,11 @@ __global__ void __launch_bounds__(WR * WK * 64, 2) kv_attention_kernel(KvAttenti
     const int b = a.row_blocks == 1 ? (int)blockIdx.z : (int)blockIdx.z / a.row_blocks, rb = (int)blockIdx.z - b * a.row_blocks;
     const int G = a.n_q / a.H, rows = a.T * G;
     const int start = min(a.start[b], a.cap);
-    const int n = start < 0 ? 0 : min(start + a.T, a.cap);                   // rows of the cache that exist
+    const int n = kv_rows(start, a.T, a.cap);
     const int blocks = (n + 63) >> 6;
     const int per = (blocks + a.splits - 1) / a.splits;
     const int lo = split * per, hi = min(lo + per, blocks);
+    if (split > 0 && lo >= hi) return;                                       // nothing left for this split: the join leaves it out too
     const size_t plane = ((size_t)b * a.H + hk) * a.cap;
     // lane addresses of block 0
     const uint8_t* kc = a.kc + (plane + 16 * (c >> 2) + (c & 3)) * D + 16 * j;
@@ -481,20 +489,21 @@ __global__ void __launch_bounds__(WR * WK * 64, 2) kv_attention_kernel(KvAttenti
     }
 }
 
-// joins the splits of one output row: 256 / (D / 4) of them at a time, four channels a lane, and these sums in order
+// joins the splits of one output row (grid: rows of a sequence, sequences): 256 / (D / 4) of them at a time, four channels a lane, and these sums in order
 template <int D>
-__global__ void __launch_bounds__(256) kv_attention_join_kernel(const float* part_o, const float* part_ml, bf16* out, int splits) {
+__global__ void __launch_bounds__(256) kv_attention_join_kernel(const float* part_o, const float* part_ml, bf16* out, const int* start, int T, int cap,
+                                                                int splits) {
     constexpr int LPR = D / 4, P = 256 / LPR;
     __shared__ f32x4 lds_y[P][LPR];
     __shared__ float lds_s[P];
-    const size_t row = blockIdx.x;
+    const size_t row = (size_t)blockIdx.y * gridDim.x + blockIdx.x;
     const int tid = (int)threadIdx.x, p = tid / LPR, l = tid % LPR;
     const float* ml = part_ml + row * splits * 2;
     const float* po = part_o + row * splits * D + 4 * l;
     float mx = -INFINITY;
     f32x4 y = {};
     float sum = 0.f;
-    // the first eight splits of a lane are on their way before the maximum over all splits is taken
+    // the first eight splits of a lane are on their way before their number and the maximum over all of them are known: what no split wrote is not used
     f32x4 x[8];
     f32x2 t[8];
 #pragma unroll
@@ -503,7 +512,10 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const float* par
         x[u] = *(const f32x4*)(po + (size_t)s * D);
         t[u] = *(const f32x2*)(ml + 2 * s);
     }
-    for (int s = tid & 63; s < splits; s += 64) mx = fmaxf(mx, ml[2 * s]);
+    const float m0 = ml[2 * min(tid & 63, splits - 1)];
+    const int used = kv_used_splits(start[blockIdx.y], T, cap, splits);
+    if ((tid & 63) < used) mx = fmaxf(mx, m0);
+    for (int s = (tid & 63) + 64; s < used; s += 64) mx = fmaxf(mx, ml[2 * s]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
     auto add = [&](const f32x4& v, const f32x2& w) __attribute__((always_inline)) {
@@ -514,8 +526,8 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const float* par
     };
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-        if (p + u * P < splits) add(x[u], t[u]);
-    for (int s = p + 8 * P; s < splits; s += P) add(*(const f32x4*)(po + (size_t)s * D), *(const f32x2*)(ml + 2 * s));
+        if (p + u * P < used) add(x[u], t[u]);
+    for (int s = p + 8 * P; s < used; s += P) add(*(const f32x4*)(po + (size_t)s * D), *(const f32x2*)(ml + 2 * s));
     // a split that saw nothing has m = -inf and weight 0 -- or, where every score is NaN, sums of NaN: they stay
     lds_y[p][l] = y;
     if (l == 0) lds_s[p] = sum;
@@ -532,9 +544,12 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const float* par
     *(bf16x4*)(out + row * D + 4 * l) = z;
 }
 
-// How the work is cut: row tiles of a work-group, row blocks, splits of the cache's axis.  One work-group per CU wants 256 of them; more splits than
-// that only add partials to join (8 sequences' heads, 30000 rows: 32 splits 19.9 us, 64 21.4, 117 25.4) -- except where the sequences of a batch
-// differ in length and the longest would be left over: 24 x 8 heads, 0 ... 40000 rows: 2 splits 153 us, 3 115, 6 98, 11 96.  A split is never shorter
+// How the work is cut: row tiles of a work-group, row blocks, splits of the cache's axis.  One work-group per CU is 256 of them, no more (21 rows a head,
+// 12 work-groups, 15000 cache rows: 21 splits 25.6 us, 22 31.4); more splits than that only add partials to join (8 sequences' heads, 30000 rows: 32
+// splits 19.9 us, 64 21.4, 117 25.4) -- except where the sequences of a batch differ in length and the longest would be left over: 24 x 8 heads,
+// 0 ... 40000 rows: 2 splits 153 us, 3 115, 6 98, 11 96, and where several row tiles walk far: their steps are chains of dependent instructions, and a
+// second work-group on the CU fills the gaps (33 tokens, 2 x 4 heads, 12000 rows: 8 splits 42.3 us, 16 28.6; 64 tokens, 4 heads, 15000 rows: 9 46.1, 18
+// 42.6; not below four blocks a wave: 3 trees of 21, 2777 rows: 8 20.7, 14 21.9).  A split is never shorter
 // than one block of 64 rows for each wave that shares the cache, and two where none do (21 rows a head, cap 1536: 128 rows 9.2 us, 256 10.8).
 struct KvPlan { int wr, rb, splits; };
 static KvPlan kv_plan(int B, int H, int T, int n_q, int cap) {
@@ -542,8 +557,9 @@ static KvPlan kv_plan(int B, int H, int T, int n_q, int cap) {
     const int rows = T * (n_q / H);
     p.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     p.rb = (rows + 16 * p.wr - 1) / (16 * p.wr);
-    const long long wgs = (long long)B * H * p.rb, fill = (256 + wgs - 1) / wgs, even = (2048 + wgs - 1) / wgs;
-    const long long s = fill > 8 ? fill : even < 8 ? even : 8;
+    const long long wgs = (long long)B * H * p.rb, one = 256 / wgs, two = 512 / wgs, even = (2048 + wgs - 1) / wgs;
+    long long s = one > 8 ? one : even < 8 ? even : 8;
+    if (p.wr > 1 && two > s && cap / 64 >= 4 * (4 / p.wr) * two) s = two;
     const int most = (cap + (p.wr == 1 ? 255 : 127)) / (p.wr == 1 ? 256 : 128);
     p.splits = (int)(s < most ? s : most);
     return p;
@@ -581,8 +597,9 @@ int launch_kv_attention(const KvAttention& in, void* workspace, size_t workspace
 #undef PE_KV_ATT
     if (const int rc = check_launch("kv_attention_kernel")) return rc;
     if (a.splits > 1) {
-        if (a.D == 64) hipLaunchKernelGGL(kv_attention_join_kernel<64>, dim3((unsigned)out_rows), dim3(256), 0, stream, a.part_o, a.part_ml, a.out, a.splits);
-        else hipLaunchKernelGGL(kv_attention_join_kernel<128>, dim3((unsigned)out_rows), dim3(256), 0, stream, a.part_o, a.part_ml, a.out, a.splits);
+        const dim3 rows(a.T * a.n_q, a.B);
+        if (a.D == 64) hipLaunchKernelGGL(kv_attention_join_kernel<64>, rows, dim3(256), 0, stream, a.part_o, a.part_ml, a.out, a.start, a.T, a.cap, a.splits);
+        else hipLaunchKernelGGL(kv_attention_join_kernel<128>, rows, dim3(256), 0, stream, a.part_o, a.part_ml, a.out, a.start, a.T, a.cap, a.splits);
         return check_launch("kv_attention_join_kernel");
     }
     return PE_OK;

@@ -467,6 +467,22 @@ def test_kv_attention(ops, B, T, hq, hkv, D, cap, starts, mask):
         assert torch.equal(ops.kv_attention_e4m3(q, cache, start, tree=bits_.long().expand(B, T).contiguous()), got)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [1, 3, 5, 40])                       # 7, 21, 35, 280 rows a kv head: one, two, four row tiles, several blocks of them
+def test_kv_attention_short_prefixes_in_a_long_cache(ops, T, D):
+    """splits that have no rows write nothing, and what the workspace held before is not read into any result"""
+    g = gen(D + T)
+    B, hq, hkv, cap = 5, 14, 2, 8192
+    cache = filled(ops, g, B, hkv, cap, D)
+    q = (1.5 * randn(g, B, T, hq, D)).to(BF)
+    start = torch.tensor([0, 100, 5000, -1, 64 * 20 - T], dtype=torch.int32, device="cuda")
+    ws = ops.kv_attention_workspace(cache, T, hq)
+    assert ws.numel() > 0
+    got = [ops.kv_attention_e4m3(q, cache, start, workspace=ws.fill_(fill)) for fill in (255, 127, 0)]      # NaN, large numbers, zeros
+    near(got[0], *attention_reference(q, cache, start))
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2]) and (got[0][3] == 0).all()
+
+
 def test_kv_attention_masked_rows_do_not_leak(ops):
     """rows that are not finite, or anything at all behind the last token: no influence where masked, NaN where seen"""
     g = gen(12)
