@@ -320,6 +320,24 @@ def accelerate_decode(model) -> int:
     return n
 
 
+# what a generation config can hold beside the penalty, the suppressed tokens and the least length that the captured step applies itself, and makes
+# transformers' generate() choose other tokens, more of them or fewer: (name, the values that change nothing)
+_OTHER_CHOICES = (
+    ("do_sample", (None, False)), ("num_beams", (None, 1)), ("num_beam_groups", (None, 1)), ("num_return_sequences", (None, 1)), ("diversity_penalty", (None, 0.0)),
+    ("constraints", (None,)), ("force_words_ids", (None,)), ("no_repeat_ngram_size", (None, 0)), ("encoder_no_repeat_ngram_size", (None, 0)),
+    ("encoder_repetition_penalty", (None, 1.0)), ("bad_words_ids", (None, [])), ("sequence_bias", (None, [], {})), ("begin_suppress_tokens", (None, [])),
+    ("forced_bos_token_id", (None,)), ("forced_eos_token_id", (None,)), ("exponential_decay_length_penalty", (None,)), ("remove_invalid_values", (None, False)),
+    ("guidance_scale", (None, 1.0)), ("watermarking_config", (None,)), ("token_healing", (None, False)), ("stop_strings", (None, [])), ("max_time", (None,)),
+    ("penalty_alpha", (None, 0.0)), ("dola_layers", (None,)), ("prompt_lookup_num_tokens", (None, 0)))
+
+
+def _captured_step_covers(gen) -> bool:
+    """whether GraphDecoder makes the choices that this generation config asks for: greedy, with at most a repetition penalty, suppressed tokens and a
+    least number of tokens"""
+    penalty = getattr(gen, "repetition_penalty", None)
+    return ((penalty is None or float(penalty) > 0.0) and all(getattr(gen, name, None) in neutral for name, neutral in _OTHER_CHOICES))
+
+
 class GraphDecoder:
     """Greedy `generate` of the text encoder (qwen_image_physical.py:859-873: `text_encoder.generate(**model_inputs,
     max_new_tokens=1000)`, greedy by the model's generation config) with the whole decode step -- embedding row, 28 decoder layers
@@ -337,8 +355,9 @@ class GraphDecoder:
     `w4_group` inputs (pe_gemv_w4: a quarter of the weight bytes; q / k / v and gate / up are one matrix each, the RMSNorm weights folded into
     their columns).  The copies are made at the first call from the model's weights and again when those move or change (call reset() after
     changing them through `.data`, or weights made under inference_mode: nothing counts those changes).
-    Penalties and masks: a repetition_penalty or suppress_tokens of the generation config, or generate(prefix_allowed_tokens_fn=), make the
-    next token the first maximum of the processed scores (pe_select_token) instead of the plain arg-max."""
+    Penalties and masks: a repetition_penalty, suppress_tokens, min_new_tokens or min_length (no EOS before) of the generation config, or
+    generate(prefix_allowed_tokens_fn=), make the next token the first maximum of the processed scores (pe_select_token) instead of the plain
+    arg-max.  Nothing else of the config is applied here: PromptPrologue.generate_ids hands a config that asks for more to transformers."""
 
     MAX_CACHE_ROWS = 15360          # rows of the static K / V planes pe_decode_step_attention can walk
 
@@ -487,8 +506,8 @@ class GraphDecoder:
         return ops.gemv_norm(x, self.lm.norm.weight, float(self.lm.norm.variance_epsilon), self.model.lm_head.weight,
                              self.model.lm_head.bias)
 
-    def _allow(self, st, ids):
-        """the mask of allowed tokens: all (None) or the given ids, without the generation config's suppress_tokens"""
+    def _allow(self, st, ids, without=()):
+        """the mask of allowed tokens: all (None) or the given ids, without the generation config's suppress_tokens and the ids of `without`"""
         V = st["counts"].shape[1]
         bits = torch.full((V + 31,), ids is None, dtype=torch.bool)
         if ids is not None:
@@ -496,7 +515,7 @@ class GraphDecoder:
             if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= V):
                 raise ValueError(f"prefix_allowed_tokens_fn: token ids outside 0 ... {V - 1}")
             bits[ids] = True
-        gone = [t for t in (getattr(self.model.generation_config, "suppress_tokens", None) or ()) if 0 <= t < V]
+        gone = [t for t in (*(getattr(self.model.generation_config, "suppress_tokens", None) or ()), *without) if 0 <= t < V]
         bits[torch.as_tensor(gone, dtype=torch.long)] = False
         words = (bits[:V + (-V) % 32].view(-1, 32).long() << torch.arange(32)).sum(1)
         st["allowed"].copy_(torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32))
@@ -514,9 +533,11 @@ class GraphDecoder:
         gen = model.generation_config
         eos = gen.eos_token_id
         eos = set() if eos is None else set(eos if isinstance(eos, (list, tuple)) else [eos])
-        min_new = int(getattr(gen, "min_new_tokens", 0) or 0)
+        # EOS is not allowed among the first min_new tokens; min_length, which counts the prompt, holds where min_new_tokens is not given
+        min_new = getattr(gen, "min_new_tokens", None)
+        min_new = max(int(getattr(gen, "min_length", None) or 0) - Lp if min_new is None else int(min_new), 0) if eos else 0
         penalty = float(getattr(gen, "repetition_penalty", None) or 1.0)
-        select = prefix_allowed_tokens_fn is not None or penalty != 1.0 or bool(getattr(gen, "suppress_tokens", None))
+        select = prefix_allowed_tokens_fn is not None or penalty != 1.0 or bool(getattr(gen, "suppress_tokens", None)) or min_new > 0
         cap = Lp + max_new_tokens
         if cap > self.MAX_CACHE_ROWS:
             raise ValueError(f"GraphDecoder.generate: prompt + max_new_tokens exceeds the decode attention's {self.MAX_CACHE_ROWS}-row cache")
@@ -587,7 +608,7 @@ class GraphDecoder:
             st["counts"].zero_()
             self.ops.token_counts_add(st["counts"], ids.to(device=dev, dtype=torch.int32).contiguous(), prompt=True)
             st["penalties"].copy_(torch.tensor([penalty, 0.0, 0.0]))
-            self._allow(st, prefix_allowed_tokens_fn(0, ids[0]) if prefix_allowed_tokens_fn else None)
+            self._allow(st, prefix_allowed_tokens_fn(0, ids[0]) if prefix_allowed_tokens_fn else None, eos if min_new else ())
             first = int(self.ops.select_token(last_logits, counts=st["counts"], penalties=st["penalties"], allowed=st["allowed"], update_counts=True))
             if first < 0:
                 raise RuntimeError("GraphDecoder.generate: no token is allowed")
@@ -603,7 +624,7 @@ class GraphDecoder:
         st["sin"][Lp:Lp + max_new_tokens].copy_(sin[:, 0].permute(1, 0, 2)[:, self.sel, ar].to(torch.bfloat16))
         tokens = [first]
         n_steps = max_new_tokens - 1                       # the prefill produced the first new token
-        if n_steps > 0 and not (first in eos and min_new <= 1):
+        if n_steps > 0 and first not in eos:
             side = torch.cuda.Stream(device=dev)
             side.wait_stream(torch.cuda.current_stream(dev))
             with torch.cuda.stream(side):
@@ -623,11 +644,18 @@ class GraphDecoder:
                 graph = st["graph"]
                 st["step"].fill_(Lp)
                 st["token"].fill_(first)
-                done = 0
+                done, no_eos = 0, min_new > 0
                 while done < n_steps:
                     n = min(self.chunk if prefix_allowed_tokens_fn is None else 1, n_steps - done)
+                    early = done + 1 < min_new                                       # the next token is generated token done + 1
+                    if early:
+                        n = min(n, min_new - done - 1)                               # the mask changes in between
                     if prefix_allowed_tokens_fn is not None:
-                        self._allow(st, prefix_allowed_tokens_fn(0, torch.cat([ids[0], torch.tensor(tokens, dtype=ids.dtype, device=ids.device)])))
+                        self._allow(st, prefix_allowed_tokens_fn(0, torch.cat([ids[0], torch.tensor(tokens, dtype=ids.dtype, device=ids.device)])),
+                                    eos if early else ())
+                    elif no_eos and not early:
+                        self._allow(st, None)
+                        no_eos = False
                     for _ in range(n):
                         graph.replay()
                     new = st["out_ids"][Lp + done:Lp + done + n].tolist()            # synchronises
@@ -637,7 +665,7 @@ class GraphDecoder:
                     done += n
                     if select and min(new) < 0:
                         raise RuntimeError("GraphDecoder.generate: no token is allowed")
-                    stop = next((i for i, t in enumerate(new) if t in eos and len(tokens) + i + 1 >= max(min_new, 1)), None)
+                    stop = next((i for i, t in enumerate(new) if t in eos), None)
                     if stop is not None:
                         tokens += new[:stop + 1]
                         break
@@ -784,18 +812,16 @@ class PromptPrologue:
     @torch.no_grad()
     def generate_ids(self, model_inputs, max_new_tokens: int, prefix_allowed_tokens_fn=None):
         """`text_encoder.generate(**model_inputs, max_new_tokens=...)`: through the captured decode step when the encoder qualifies
-        (bf16 on the GPU, greedy; a repetition penalty, suppressed tokens and a callback for the allowed ones included), through
-        transformers otherwise."""
+        (bf16 on the GPU, greedy; a repetition penalty, suppressed tokens, a least number of tokens and a callback for the allowed ones
+        included), through transformers otherwise."""
         gen = self.text_encoder.generation_config
-        plain_greedy = (not getattr(gen, "do_sample", False) and (getattr(gen, "num_beams", 1) or 1) == 1
-                        and (getattr(gen, "repetition_penalty", None) or 1.0) > 0.0
-                        and not getattr(gen, "no_repeat_ngram_size", 0) and not getattr(gen, "bad_words_ids", None)
-                        and not getattr(gen, "forced_eos_token_id", None))
         ids = model_inputs["input_ids"]
-        if (self.graph_decoder is not None and plain_greedy and ids.shape[0] == 1
+        if (self.graph_decoder is not None and _captured_step_covers(gen) and ids.shape[0] == 1
                 and ids.shape[1] + max_new_tokens <= GraphDecoder.MAX_CACHE_ROWS):        # longer: the reference's own path
             return self.graph_decoder.generate(max_new_tokens=max_new_tokens, prefix_allowed_tokens_fn=prefix_allowed_tokens_fn, **model_inputs)
         more = {} if prefix_allowed_tokens_fn is None else {"prefix_allowed_tokens_fn": prefix_allowed_tokens_fn}
+        if getattr(gen, "stop_strings", None):
+            more["tokenizer"] = self.tokenizer
         return self.text_encoder.generate(**model_inputs, max_new_tokens=max_new_tokens, **more)
 
     def physical_text(self, prompt: str, edit_image: Image.Image) -> str:

@@ -1,0 +1,66 @@
+"""CPU checks of which path PromptPrologue decodes on: the captured step only for what it applies itself, transformers for the rest."""
+import types
+
+import pytest
+import torch
+from transformers import GenerationConfig
+
+from diffsynth.pipelines import prompt_prologue as PP
+
+
+class Recorder:
+    """stands for the captured decoder and for the text encoder: notes which of them was asked, and how"""
+    max_rows = PP.GraphDecoder.MAX_CACHE_ROWS
+
+    def __init__(self, calls, name):
+        self.calls, self.name = calls, name
+
+    def generate(self, **kw):
+        self.calls.append((self.name, kw))
+        return kw["input_ids"]
+
+
+def prologue(**config):
+    calls = []
+    pp = PP.PromptPrologue.__new__(PP.PromptPrologue)
+    pp.text_encoder, pp.graph_decoder, pp.tokenizer = Recorder(calls, "transformers"), Recorder(calls, "captured"), "the tokenizer"
+    pp.text_encoder.generation_config = GenerationConfig(eos_token_id=2, pad_token_id=0, **config)
+    return pp, calls
+
+
+INPUTS = dict(input_ids=torch.zeros((1, 5), dtype=torch.long))
+OTHERS = [dict(do_sample=True), dict(num_beams=2), dict(no_repeat_ngram_size=2), dict(bad_words_ids=[[3]]), dict(forced_eos_token_id=2), dict(forced_eos_token_id=0),
+          dict(begin_suppress_tokens=[4]), dict(sequence_bias=[[[4], 1.0]]), dict(encoder_repetition_penalty=1.2), dict(encoder_no_repeat_ngram_size=2),
+          dict(forced_bos_token_id=0), dict(exponential_decay_length_penalty=(3, 1.1)), dict(remove_invalid_values=True), dict(guidance_scale=1.5),
+          dict(max_time=1.0), dict(prompt_lookup_num_tokens=3)]
+
+
+@pytest.mark.parametrize("more", OTHERS, ids=lambda d: next(iter(d)))
+@pytest.mark.parametrize("penalty", [dict(), dict(repetition_penalty=1.3), dict(suppress_tokens=[7])], ids=["plain", "penalty", "suppressed"])
+def test_what_the_captured_step_does_not_apply_goes_to_transformers(more, penalty):
+    pp, calls = prologue(**more, **penalty)
+    pp.generate_ids(INPUTS, 9)
+    assert [c[0] for c in calls] == ["transformers"] and calls[0][1]["max_new_tokens"] == 9
+
+
+@pytest.mark.parametrize("config", [dict(), dict(repetition_penalty=1.3), dict(suppress_tokens=[7, 8]), dict(min_new_tokens=4), dict(min_length=9, repetition_penalty=0.8),
+                                    dict(temperature=0.1, top_k=1, top_p=0.5, do_sample=False, num_beams=1, guidance_scale=1.0, no_repeat_ngram_size=0)])
+def test_what_the_captured_step_applies_stays_there(config):
+    pp, calls = prologue(**config)
+    grammar = lambda b, ids: [3]
+    pp.generate_ids(INPUTS, 9)
+    pp.generate_ids(INPUTS, 9, prefix_allowed_tokens_fn=grammar)
+    assert [(c[0], c[1]["prefix_allowed_tokens_fn"]) for c in calls] == [("captured", None), ("captured", grammar)]
+
+
+def test_stop_strings_come_with_the_tokenizer():
+    pp, calls = prologue(stop_strings=["."])
+    pp.generate_ids(INPUTS, 9)
+    assert calls[0][0] == "transformers" and calls[0][1]["tokenizer"] == "the tokenizer" and "prefix_allowed_tokens_fn" not in calls[0][1]
+
+
+def test_a_penalty_that_is_none_at_all_is_refused_by_transformers():
+    pp, calls = prologue()
+    pp.text_encoder.generation_config = types.SimpleNamespace(repetition_penalty=0.0)
+    pp.generate_ids(INPUTS, 9)
+    assert calls[0][0] == "transformers"

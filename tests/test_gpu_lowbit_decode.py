@@ -252,3 +252,32 @@ def test_a_tree_of_drafts_equals_its_branches(model):
             assert torch.equal(one[0, 0], qr[0, i])
             # the same numbers in another order of sums, each rounded once: half a step apart on either side
             assert ((got[0, i].float() - alone[0, 0].float()).abs() <= 2.0 ** -7 * alone[0, 0].float().abs() + 2.0 ** -14).all()
+
+
+@pytest.mark.parametrize("penalty", [1.0, 1.3])
+def test_no_eos_before_the_least_number_of_tokens(model, config, penalty):
+    """min_new_tokens and min_length keep EOS out of the first tokens and out of the cache, as transformers does; it ends the answer after them"""
+    dec = decoder(model)
+    inputs = prompt(37)
+    config.repetition_penalty = penalty
+    free = dec.generate(max_new_tokens=24, **inputs)[0, 37:].tolist()
+    stops = 0
+    for least in (dict(min_new_tokens=1), dict(min_new_tokens=5), dict(min_new_tokens=11), dict(min_length=37 + 3), dict(min_length=30), dict(min_new_tokens=2, min_length=50),
+                  dict(min_new_tokens=0, min_length=50), dict(min_new_tokens=24)):
+        for eos in ([free[0]], [free[2], free[6]], [free[0], free[1], free[12]]):
+            config.eos_token_id, config.min_new_tokens, config.min_length = eos, least.get("min_new_tokens"), least.get("min_length")
+            with torch.no_grad():
+                want = model.generate(**inputs, max_new_tokens=24)
+            got = dec.generate(max_new_tokens=24, **inputs)
+            assert torch.equal(got, want), (least, eos)
+            early = least.get("min_new_tokens", max(least.get("min_length", 0) - 37, 0))
+            assert not set(got[0, 37:37 + early].tolist()) & set(eos)
+            stops += got.shape[1] < 37 + 24
+    assert stops > 0
+    # with a grammar in force too
+    config.eos_token_id, config.min_new_tokens, config.min_length = [500], 4, None
+    with torch.no_grad():
+        want = model.generate(**inputs, max_new_tokens=8, prefix_allowed_tokens_fn=lambda b, i: [500, 501 + i.numel()])
+    assert torch.equal(dec.generate(max_new_tokens=8, prefix_allowed_tokens_fn=lambda b, i: [500, 501 + i.numel()], **inputs), want)
+    config.eos_token_id, config.min_new_tokens = None, 5                     # no EOS: nothing to keep out
+    assert dec.generate(max_new_tokens=24, **inputs)[0, 37:].tolist() == free
