@@ -832,7 +832,8 @@ class PromptPrologue:
         ]
         text = self.processor.apply_chat_template(messages, tokenize=False, add_generation_prompt=True, add_vision_id=True)
         model_inputs = self.processor(text=[text], images=resize_for_vl(edit_image), padding=True, return_tensors="pt").to(self.device)
-        decoded_ids = self.generate_ids(model_inputs, max_new_tokens=1000, prefix_allowed_tokens_fn=self.allowed_tokens_fn)
+        grammar = {} if self.allowed_tokens_fn is None else {"prefix_allowed_tokens_fn": self.allowed_tokens_fn}
+        decoded_ids = self.generate_ids(model_inputs, max_new_tokens=1000, **grammar)
         trimmed = [out_ids[len(in_ids):] for in_ids, out_ids in zip(model_inputs["input_ids"], decoded_ids)]
         decoded = self.tokenizer.batch_decode(trimmed, skip_special_tokens=True, clean_up_tokenization_spaces=False)[0]
         try:

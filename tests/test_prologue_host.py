@@ -99,3 +99,17 @@ def test_text_encoder_key_conversion():
           "model.language_model.norm.weight": torch.zeros(1), "lm_head.weight": torch.zeros(1)}
     assert set(PP.convert_text_encoder_keys(sd)) == {"model.visual.blocks.0.attn.qkv.weight", "model.language_model.layers.0.mlp.up_proj.weight",
                                                      "model.language_model.norm.weight", "lm_head.weight"}
+
+
+def test_generate_ids_may_be_replaced_by_one_of_two_arguments(prologue, monkeypatch):
+    """a program's own generate_ids(model_inputs, max_new_tokens) still serves where no grammar is set; with one it is asked for the grammar too"""
+    real, asked = PP.PromptPrologue.generate_ids, []
+
+    def short(self, model_inputs, max_new_tokens):
+        asked.append(max_new_tokens)
+        return real(self, model_inputs, 3)
+    monkeypatch.setattr(PP.PromptPrologue, "generate_ids", short)
+    assert isinstance(prologue.physical_text("tilt the glass", tiny_vl.make_image(64, 64, 9)), str) and asked == [1000]
+    monkeypatch.setattr(prologue, "allowed_tokens_fn", lambda b, ids: [5])
+    with pytest.raises(TypeError):
+        prologue.physical_text("tilt the glass", tiny_vl.make_image(64, 64, 9))
