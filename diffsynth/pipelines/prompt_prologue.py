@@ -894,7 +894,7 @@ class PromptPrologue:
         clone = lambda d: {k: (v.clone() if isinstance(v, torch.Tensor) else v) for k, v in d.items()}   # callers mutate prompt_emb
         gen = getattr(self.text_encoder, "generation_config", None)
         key = (prompt, negative_prompt, self._image_key(edit_image), bool(cfg), bool(have_text_reasoning), physical_txt,
-               getattr(gen, "repetition_penalty", None), tuple(getattr(gen, "suppress_tokens", None) or ()))
+               repr(sorted(vars(gen).items())) if gen is not None else None)          # the answer is the config's too: penalties, EOS, lengths
         given = physical_txt
         cache_size = self.cache_size if self.allowed_tokens_fn is None else 0          # a callback's answers are its own
         if cache_size and key in self._cache:

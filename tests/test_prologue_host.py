@@ -113,3 +113,21 @@ def test_generate_ids_may_be_replaced_by_one_of_two_arguments(prologue, monkeypa
     monkeypatch.setattr(prologue, "allowed_tokens_fn", lambda b, ids: [5])
     with pytest.raises(TypeError):
         prologue.physical_text("tilt the glass", tiny_vl.make_image(64, 64, 9))
+
+
+@pytest.mark.parametrize("field,value", [("repetition_penalty", 1.4), ("suppress_tokens", [3, 4]), ("min_new_tokens", 4), ("min_length", 400), ("eos_token_id", [3, 5]),
+                                         ("no_repeat_ngram_size", 2), ("begin_suppress_tokens", [7])])
+def test_a_changed_generation_config_is_not_answered_from_the_cache(prologue, monkeypatch, field, value):
+    answers = iter("abc")
+    monkeypatch.setattr(prologue, "physical_text", lambda *a: next(answers))
+    gen = prologue.text_encoder.generation_config
+    kw = dict(prompt="melt the ice", negative_prompt="", edit_image=tiny_vl.make_image(96, 64, 5), cfg=False)
+    prologue._cache.clear()
+    first = prologue(None, **kw)[0]["prompt_emb"]
+    assert prologue.last_physical_txt == "a" and torch.equal(prologue(None, **kw)[0]["prompt_emb"], first) and prologue.last_physical_txt == "a"
+    monkeypatch.setattr(gen, field, value)
+    prologue(None, **kw)
+    assert prologue.last_physical_txt == "b"
+    monkeypatch.undo()
+    prologue(None, **kw)
+    assert prologue.last_physical_txt == "a"                     # the first config's answer is still there
