@@ -361,11 +361,15 @@ class GraphDecoder:
 
     MAX_CACHE_ROWS = 15360          # rows of the static K / V planes pe_decode_step_attention can walk
 
+    @staticmethod
+    def choice(weights: Optional[str] = None, kv_cache: Optional[str] = None) -> Tuple[str, str]:
+        """(weights, kv_cache) in force: the arguments, else the environment's PE_DECODE_WEIGHTS / PE_DECODE_KV_CACHE, else bf16"""
+        return weights or os.environ.get("PE_DECODE_WEIGHTS") or "bf16", kv_cache or os.environ.get("PE_DECODE_KV_CACHE") or "bf16"
+
     def __init__(self, model, chunk: int = 16, weights: Optional[str] = None, kv_cache: Optional[str] = None, w4_group: int = 128):
         from physicedit_amd import ops
         self.ops, self.model, self.chunk = ops, model, chunk
-        self.weights = weights or os.environ.get("PE_DECODE_WEIGHTS", "bf16")
-        self.kv_cache = kv_cache or os.environ.get("PE_DECODE_KV_CACHE", "bf16")
+        self.weights, self.kv_cache = self.choice(weights, kv_cache)
         self.w4_group = w4_group
         if self.weights not in ("bf16", "w4") or self.kv_cache not in ("bf16", "e4m3") or (self.weights == "w4" and self.kv_cache != "e4m3"):
             raise ValueError(f"GraphDecoder: weights={self.weights!r}, kv_cache={self.kv_cache!r} (bf16 and bf16, bf16 and e4m3, or w4 and e4m3)")
@@ -754,7 +758,9 @@ class PromptPrologue:
     def __init__(self, text_encoder, processor, tokenizer=None, device="cuda", torch_dtype=torch.bfloat16, decode_gemv: bool = True,
                  decode_graph: bool = True, decode_weights: Optional[str] = None, decode_kv_cache: Optional[str] = None):
         """decode_weights / decode_kv_cache: GraphDecoder's weights ("bf16", "w4") and kv_cache ("bf16", "e4m3"); by default the environment's
-        PE_DECODE_WEIGHTS / PE_DECODE_KV_CACHE, else bf16."""
+        PE_DECODE_WEIGHTS / PE_DECODE_KV_CACHE, else bf16.  What is chosen there is used or refused (ValueError): only bf16 falls back to
+        transformers' generate() where the captured step is not available or switched off."""
+        low_bit = GraphDecoder.choice(decode_weights, decode_kv_cache) != ("bf16", "bf16")
         self.text_encoder = text_encoder
         self.decode_gemv = 0
         self.graph_decoder = None
@@ -764,9 +770,12 @@ class PromptPrologue:
                 try:
                     self.graph_decoder = GraphDecoder(text_encoder, weights=decode_weights, kv_cache=decode_kv_cache)
                 except (ValueError, AttributeError) as e:            # another architecture / dtype: transformers' generate()
-                    if (decode_weights or "bf16", decode_kv_cache or "bf16") != ("bf16", "bf16"):
+                    if low_bit:
                         raise                                          # asked for by name: no silent bf16
                     print(f"[prompt_prologue] captured decode step not available ({e}); using generate()")
+        if low_bit and text_encoder is not None and self.graph_decoder is None:
+            raise ValueError(f"PromptPrologue: weights, cache = {GraphDecoder.choice(decode_weights, decode_kv_cache)} are the captured decode step's, which needs "
+                             f"a GPU, decode_gemv and decode_graph (device {device}, decode_gemv={decode_gemv}, decode_graph={decode_graph})")
         self.processor = processor
         self.tokenizer = tokenizer if tokenizer is not None else processor.tokenizer
         self.device = torch.device(device)

@@ -64,3 +64,53 @@ def test_a_penalty_that_is_none_at_all_is_refused_by_transformers():
     pp.text_encoder.generation_config = types.SimpleNamespace(repetition_penalty=0.0)
     pp.generate_ids(INPUTS, 9)
     assert calls[0][0] == "transformers"
+
+
+class Processor:
+    class tokenizer:
+        convert_tokens_to_ids = staticmethod(lambda t: 5)
+
+
+def build(monkeypatch, fail=None, device="cuda", **kw):
+    """a PromptPrologue whose captured decoder is a stand-in (or fails); -> what the decoder was asked for"""
+    asked = []
+
+    class Decoder(PP.GraphDecoder):
+        def __init__(self, model, weights=None, kv_cache=None):
+            asked.append(self.choice(weights, kv_cache))
+            if fail:
+                raise ValueError(fail)
+    monkeypatch.setattr(PP, "GraphDecoder", Decoder)
+    monkeypatch.setattr(PP, "accelerate_decode", lambda m: 1)
+    pp = PP.PromptPrologue(object(), Processor(), device=device, **kw)
+    return asked, pp
+
+
+LOW = [("w4", "e4m3"), (None, "e4m3"), ("w4", None), ("int8", None)]
+
+
+@pytest.mark.parametrize("weights,cache", LOW)
+@pytest.mark.parametrize("where", ["arguments", "environment"])
+def test_a_low_bit_choice_is_used_or_refused(monkeypatch, weights, cache, where):
+    kw = {}
+    for name, var, value in (("decode_weights", "PE_DECODE_WEIGHTS", weights), ("decode_kv_cache", "PE_DECODE_KV_CACHE", cache)):
+        monkeypatch.delenv(var, raising=False)
+        if value is not None:
+            monkeypatch.setenv(var, value) if where == "environment" else kw.update({name: value})
+    asked, pp = build(monkeypatch, **kw)
+    assert asked == [(weights or "bf16", cache or "bf16")] and pp.graph_decoder is not None
+    with pytest.raises(ValueError, match="does not fit"):
+        build(monkeypatch, fail="does not fit", **kw)
+    for off in (dict(decode_graph=False), dict(decode_gemv=False), dict(device="cpu")):
+        with pytest.raises(ValueError, match="captured decode step"):
+            build(monkeypatch, **kw, **off)
+
+
+def test_bf16_falls_back(monkeypatch, capsys):
+    for var in ("PE_DECODE_WEIGHTS", "PE_DECODE_KV_CACHE"):
+        monkeypatch.delenv(var, raising=False)
+    assert build(monkeypatch, fail="another architecture")[1].graph_decoder is None and "another architecture" in capsys.readouterr().out
+    assert build(monkeypatch, decode_graph=False)[1].graph_decoder is None and build(monkeypatch, device="cpu")[1].graph_decoder is None
+    monkeypatch.setenv("PE_DECODE_WEIGHTS", "w4"), monkeypatch.setenv("PE_DECODE_KV_CACHE", "e4m3")
+    assert build(monkeypatch, decode_weights="bf16", decode_kv_cache="bf16", device="cpu")[1].graph_decoder is None       # the arguments come first
+    assert PP.PromptPrologue(None, Processor(), device="cpu").graph_decoder is None                                       # nothing to decode with
