@@ -359,7 +359,13 @@ class GraphDecoder:
     generate(prefix_allowed_tokens_fn=), make the next token the first maximum of the processed scores (pe_select_token) instead of the plain
     arg-max.  Nothing else of the config is applied here: PromptPrologue.generate_ids hands a config that asks for more to transformers."""
 
-    MAX_CACHE_ROWS = 15360          # rows of the static K / V planes pe_decode_step_attention can walk
+    MAX_CACHE_ROWS = 15360          # rows of the bf16 K / V planes pe_decode_step_attention can walk
+    MAX_CACHE_ROWS_E4M3 = 1 << 30   # KVCacheE4M3's: memory ends first
+
+    @property
+    def max_rows(self) -> int:
+        """prompt + new tokens that the captured step has room for"""
+        return self.MAX_CACHE_ROWS if self.kv_cache == "bf16" else self.MAX_CACHE_ROWS_E4M3
 
     @staticmethod
     def choice(weights: Optional[str] = None, kv_cache: Optional[str] = None) -> Tuple[str, str]:
@@ -543,8 +549,8 @@ class GraphDecoder:
         penalty = float(getattr(gen, "repetition_penalty", None) or 1.0)
         select = prefix_allowed_tokens_fn is not None or penalty != 1.0 or bool(getattr(gen, "suppress_tokens", None)) or min_new > 0
         cap = Lp + max_new_tokens
-        if cap > self.MAX_CACHE_ROWS:
-            raise ValueError(f"GraphDecoder.generate: prompt + max_new_tokens exceeds the decode attention's {self.MAX_CACHE_ROWS}-row cache")
+        if cap > self.max_rows:
+            raise ValueError(f"GraphDecoder.generate: prompt + max_new_tokens exceeds the decode attention's {self.max_rows}-row cache")
         # ---- prefill on transformers (one pass over the prompt; image tokens, mrope positions, rope_deltas are its business)
         try:
             out = model(**model_inputs, use_cache=True, logits_to_keep=1)
@@ -557,7 +563,7 @@ class GraphDecoder:
         # as an argument depends on the prompt (the cache row of generated token t is step = Lp + t, read from the device counter;
         # `base` is 0; the rotary tables are indexed by that same step), so a later call of the same bucket only refills the planes'
         # first Lp rows, the table rows [Lp, Lp + max_new_tokens) and the counter, and replays
-        bucket = min(self.MAX_CACHE_ROWS, (cap + 1023) // 1024 * 1024)
+        bucket = min(self.max_rows, (cap + 1023) // 1024 * 1024)
         st = self._static.get(bucket)
         fp = self._weights_fingerprint()
         if st is not None and st.get("weights") != fp:
@@ -826,7 +832,7 @@ class PromptPrologue:
         gen = self.text_encoder.generation_config
         ids = model_inputs["input_ids"]
         if (self.graph_decoder is not None and _captured_step_covers(gen) and ids.shape[0] == 1
-                and ids.shape[1] + max_new_tokens <= GraphDecoder.MAX_CACHE_ROWS):        # longer: the reference's own path
+                and ids.shape[1] + max_new_tokens <= self.graph_decoder.max_rows):        # longer: the reference's own path
             return self.graph_decoder.generate(max_new_tokens=max_new_tokens, prefix_allowed_tokens_fn=prefix_allowed_tokens_fn, **model_inputs)
         more = {} if prefix_allowed_tokens_fn is None else {"prefix_allowed_tokens_fn": prefix_allowed_tokens_fn}
         if getattr(gen, "stop_strings", None):

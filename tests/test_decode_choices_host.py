@@ -114,3 +114,15 @@ def test_bf16_falls_back(monkeypatch, capsys):
     monkeypatch.setenv("PE_DECODE_WEIGHTS", "w4"), monkeypatch.setenv("PE_DECODE_KV_CACHE", "e4m3")
     assert build(monkeypatch, decode_weights="bf16", decode_kv_cache="bf16", device="cpu")[1].graph_decoder is None       # the arguments come first
     assert PP.PromptPrologue(None, Processor(), device="cpu").graph_decoder is None                                       # nothing to decode with
+
+
+def test_the_caches_have_limits_of_their_own():
+    """beyond the bf16 cache's rows only the bf16 decoder leaves the captured step"""
+    long = dict(input_ids=torch.zeros((1, 15000), dtype=torch.long))
+    for kv_cache, path in (("bf16", "transformers"), ("e4m3", "captured")):
+        pp, calls = prologue()
+        pp.graph_decoder.max_rows = PP.GraphDecoder.max_rows.fget(types.SimpleNamespace(kv_cache=kv_cache, MAX_CACHE_ROWS=PP.GraphDecoder.MAX_CACHE_ROWS,
+                                                                                        MAX_CACHE_ROWS_E4M3=PP.GraphDecoder.MAX_CACHE_ROWS_E4M3))
+        pp.generate_ids(long, 1000)
+        pp.generate_ids(long, 360)
+        assert [c[0] for c in calls] == [path, "captured"]

@@ -281,3 +281,23 @@ def test_no_eos_before_the_least_number_of_tokens(model, config, penalty):
     assert torch.equal(dec.generate(max_new_tokens=8, prefix_allowed_tokens_fn=lambda b, i: [500, 501 + i.numel()], **inputs), want)
     config.eos_token_id, config.min_new_tokens = None, 5                     # no EOS: nothing to keep out
     assert dec.generate(max_new_tokens=24, **inputs)[0, 37:].tolist() == free
+
+
+def test_the_e4m3_cache_takes_long_answers(model, config):
+    """more rows than the bf16 cache's 15360: the captured step still decodes, and its tokens are those of the same step run eagerly"""
+    from diffsynth.pipelines import prompt_prologue as PP
+    pp = PP.PromptPrologue.__new__(PP.PromptPrologue)
+    pp.text_encoder, pp.graph_decoder, pp.tokenizer = model, decoder(model, kv_cache="e4m3"), None
+    dec, inputs, Lp = pp.graph_decoder, prompt(15400, 4), 15400
+    got = pp.generate_ids(inputs, 30)
+    assert dec.captures == 1 and got.shape == (1, Lp + 30) and torch.equal(got[:, :Lp], inputs["input_ids"])
+    toks = got[0, Lp:].tolist()
+    st = next(iter(dec._static.values()))
+    assert st["cap"] == 16384
+    st["step"].fill_(Lp), st["token"].fill_(toks[0])
+    for _ in range(29):
+        dec._step(st)
+    assert toks[1:] == st["out_ids"][Lp:Lp + 29].tolist()
+    plain = decoder(model)
+    with pytest.raises(ValueError, match="15360"):
+        plain.generate(max_new_tokens=30, **inputs)
