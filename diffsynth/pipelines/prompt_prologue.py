@@ -437,7 +437,6 @@ class GraphDecoder:
         """the copies that the low-bit step keeps of the weights `fp` describes: per layer q / k / v as one matrix and its bias and, for "w4", all in
         4 bits: (qkv, its bias, o, gate_up, down), and the lm_head"""
         if self._w4 is None or self._w4[0] != fp:
-            self._w4 = None                                # the old copies go before the new ones come
             w4 = self.weights == "w4"
             q4 = lambda w, norm=None: self.ops.quantize_w4(w.contiguous(), self.w4_group, norm_w=norm)
             layers = []
@@ -569,6 +568,10 @@ class GraphDecoder:
         if st is not None and st.get("weights") != fp:
             st = None                                      # the weights moved since the capture: those launches point at the old ones
         if st is None:
+            # the old graph, planes and weight copies go before the new ones come (one bucket alive at a time, 28 KiB per row of capacity and plane pair)
+            self._static = {}
+            if self._w4 is not None and self._w4[0] != fp:
+                self._w4 = None
             kc = torch.zeros((L if self.kv_cache == "bf16" else 0, self.hkv, bucket, 128), dtype=torch.bfloat16, device=dev)
             st = {"kc": kc, "base": 0, "cap": bucket, "select": False,
                   "cos": torch.zeros((bucket, 128), dtype=torch.bfloat16, device=dev),
@@ -590,7 +593,7 @@ class GraphDecoder:
                     ly.self_attn.v_proj.weight, ly.self_attn.v_proj.bias, ly.self_attn.o_proj.weight, ly.mlp.gate_proj.weight, ly.mlp.up_proj.weight,
                     ly.mlp.down_proj.weight, ly.input_layernorm.weight, ly.input_layernorm.variance_epsilon, ly.post_attention_layernorm.weight,
                     ly.post_attention_layernorm.variance_epsilon) for ly in self.layers]
-            self._static = {bucket: st}                    # one bucket alive at a time (28 KiB per row of capacity and plane pair)
+            self._static = {bucket: st}
         if select != st["select"]:       # the captured step ends in the other choice of a token
             st["graph"], st["select"] = None, select
         if select and "counts" not in st:

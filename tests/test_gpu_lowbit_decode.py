@@ -301,3 +301,37 @@ def test_the_e4m3_cache_takes_long_answers(model, config):
     plain = decoder(model)
     with pytest.raises(ValueError, match="15360"):
         plain.generate(max_new_tokens=30, **inputs)
+
+
+@pytest.mark.parametrize("weights,kv_cache", [("bf16", "bf16"), ("bf16", "e4m3"), ("w4", "e4m3")])
+def test_old_copies_go_before_new_ones_come(model, config, weights, kv_cache):
+    """after a change of the weights or of the capacity the memory of the old step is free before the new one's is taken: the peak of a call that builds the
+    step again stays at that of the call that built it first"""
+    dec = decoder(model, weights=weights, kv_cache=kv_cache)
+    config.eos_token_id = list(range(4001))                                    # the first token ends the answer
+
+    def peak(n, **inputs):
+        torch.cuda.synchronize(), torch.cuda.empty_cache(), torch.cuda.reset_peak_memory_stats()
+        dec.generate(max_new_tokens=n, **inputs)
+        torch.cuda.synchronize()
+        return torch.cuda.max_memory_allocated() - base
+    inputs = prompt(40, 9)
+    dec.generate(max_new_tokens=2, **inputs)                                   # the libraries' own workspaces
+    dec.reset()
+    base = torch.cuda.memory_allocated()
+    first = peak(8000, **inputs) if kv_cache == "bf16" else peak(60000, **inputs)
+    held = torch.cuda.memory_allocated() - base
+    assert held > 2 ** 25                                                      # planes (and copies) of a size that would show
+    head = model.lm_head.weight
+    try:
+        if kv_cache == "bf16":
+            head.data = head.data.clone()
+        else:
+            with torch.no_grad():
+                head.mul_(1.0)                                                 # a change that counts and changes nothing
+        again = peak(8000, **inputs) if kv_cache == "bf16" else peak(60000, **inputs)
+        assert again <= first + held // 8
+        other = peak(6000, **inputs) if kv_cache == "bf16" else peak(50000, **inputs)       # another capacity
+        assert other <= first + held // 8
+    finally:
+        dec.reset()
