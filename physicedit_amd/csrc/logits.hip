@@ -114,19 +114,21 @@ PE_DEV void wave_best(float& best, int& idx) {
     for (int o = 32; o > 0; o >>= 1) better(best, idx, __shfl_xor(best, o, 64), __shfl_xor(idx, o, 64));
 }
 
-// bits 0 .. 14 of a count go up by one and stop at 32767; two tokens share a 32-bit word.  Only the token's own half changes, so any
-// order of concurrent additions gives the same counts.
-PE_DEV void count_token(short* counts, int v, bool prompt) {
-    short* p = counts + v;
+// bits 0 .. 14 of a count go up and stop at 32767; prompt: bit 15 is set instead
+PE_DEV uint32_t counted(uint32_t n, int times, bool prompt) { return prompt ? n | 0x8000u : (n & 0x8000u) | (uint32_t)min((int)(n & 0x7fffu) + times, 0x7fff); }
+
+// a count that no other lane touches
+PE_DEV void count_alone(short* p, int times, bool prompt) { *p = (short)counted((uint16_t)*p, times, prompt); }
+
+// One of the two counts of a 32-bit word, both of which belong to the row.  Only its own half changes, so any order of concurrent additions gives the
+// same counts.
+PE_DEV void count_shared(short* p, bool prompt) {
     uint32_t* word = (uint32_t*)((uintptr_t)p & ~(uintptr_t)3);
     const int shift = ((uintptr_t)p & 2) ? 16 : 0;
     uint32_t old = *word, seen;
     do {
         seen = old;
-        uint32_t n = (seen >> shift) & 0xffffu;
-        if (prompt) n |= 0x8000u;
-        else if ((n & 0x7fffu) != 0x7fffu) n += 1;
-        old = atomicCAS(word, seen, (seen & ~(0xffffu << shift)) | (n << shift));
+        old = atomicCAS(word, seen, (seen & ~(0xffffu << shift)) | (counted((seen >> shift) & 0xffffu, 1, prompt) << shift));
     } while (old != seen);
 }
 
@@ -134,7 +136,7 @@ PE_DEV void count_token(short* counts, int v, bool prompt) {
 PE_DEV void take_token(int idx, size_t row, int* token, short* counts, long long ldc, int* out_ids, int* step, int max_steps) {
     const int t = idx == NONE ? -1 : idx;
     token[row] = t;
-    if (counts && t >= 0) count_token(counts + row * ldc, t, false);
+    if (counts && t >= 0) count_alone(counts + row * ldc + t, 1, false);       // this lane writes the row's only count
     if (step) {                                   // one row only: the decode step's counter
         const int st = *step;
         if (st >= 0 && st < max_steps) out_ids[st] = t;
@@ -185,12 +187,37 @@ __global__ void __launch_bounds__(64) select_join_kernel(const float* part_v, co
     if (lane_id() == 0) take_token(idx, row, token, counts, ldc, out_ids, step, max_steps);
 }
 
-__global__ void __launch_bounds__(256) token_counts_add_kernel(short* counts, long long ldc, int V, const int* tokens, int n, int prompt) {
+// A row whose counts begin or end in the middle of a 32-bit word shares that word with the row beside it or with memory that is not the caller's: the
+// row's first work-group counts how often that one token comes and writes its 16 bits alone.  (One row of 151937, 15000 tokens: 15 loads of a lane.)
+constexpr int COUNT_THREADS = 1024;
+__global__ void __launch_bounds__(COUNT_THREADS) token_counts_add_kernel(short* counts, long long ldc, int V, const int* tokens, int n, int prompt) {
+    __shared__ int times[2];
     const size_t row = blockIdx.y;
-    const int i = (int)(blockIdx.x * 256 + threadIdx.x);
-    if (i >= n) return;
-    const int v = tokens[row * n + i];
-    if (v >= 0 && v < V) count_token(counts + row * ldc, v, prompt != 0);
+    const int tid = (int)threadIdx.x;
+    short* c = counts + row * ldc;
+    tokens += row * n;
+    const bool head = ((uintptr_t)c & 2) != 0, tail = ((uintptr_t)(c + V) & 2) != 0;       // tokens 0 and V - 1; for V = 1 at most one of them
+    const long long i = (long long)blockIdx.x * COUNT_THREADS + tid;
+    if (i < n) {
+        const int v = tokens[i];
+        if (v >= 0 && v < V && !(head && v == 0) && !(tail && v == V - 1)) count_shared(c + v, prompt != 0);
+    }
+    if (blockIdx.x != 0 || !(head || tail)) return;                                        // the whole work-group leaves
+    if (tid < 2) times[tid] = 0;
+    __syncthreads();
+    int first = 0, last = 0;
+#pragma unroll 4
+    for (long long k = tid; k < n; k += COUNT_THREADS) {
+        const int v = tokens[k];
+        first += v == 0;
+        last += v == V - 1;
+    }
+    if (first) atomicAdd(&times[0], first);
+    if (last) atomicAdd(&times[1], last);
+    __syncthreads();
+    if (tid != 0) return;
+    if (head && times[0]) count_alone(c, times[0], prompt != 0);
+    if (tail && times[1]) count_alone(c + V - 1, times[1], prompt != 0);
 }
 
 static int check_logits(const LogitsArgs& a, const char* who) {
@@ -250,7 +277,8 @@ int launch_select_token(const LogitsArgs& a, int* token, short* count_into, int*
 int launch_token_counts_add(short* counts, long long ldc, int rows, int V, const int* tokens, int n, int prompt, hipStream_t stream) {
     PE_REQUIRE(counts && tokens && ((uintptr_t)counts & 1) == 0 && ((uintptr_t)tokens & 3) == 0, "token_counts_add: null or unaligned pointer");
     PE_REQUIRE(rows >= 1 && rows <= 65535 && V >= 1 && n >= 1 && ldc >= V, "token_counts_add: bad shape (%d rows of %d, %d tokens)", rows, V, n);
-    hipLaunchKernelGGL(token_counts_add_kernel, dim3((n + 255) / 256, rows), dim3(256), 0, stream, counts, ldc, V, tokens, n, prompt);
+    hipLaunchKernelGGL(token_counts_add_kernel, dim3((unsigned)(((long long)n + COUNT_THREADS - 1) / COUNT_THREADS), rows), dim3(COUNT_THREADS), 0, stream, counts, ldc,
+                       V, tokens, n, prompt);
     return check_launch("token_counts_add_kernel");
 }
 

@@ -788,3 +788,55 @@ def test_results_over_their_inputs(ops):
     for out, out_ids, step in ((ids[:1], ids[:4], ids[5:6]), (ids[5:6], ids[:4], ids[5:6]), (ids[6:7], ids[:4], ids[3:4])):
         with pytest.raises(ValueError, match="overlaps"):
             ops.select_token(x[:1], out=out, out_ids=out_ids, step=step)
+
+
+@pytest.mark.parametrize("V", [1, 2, 7, 33, 1000, 1001])
+@pytest.mark.parametrize("R", [1, 3])
+@pytest.mark.parametrize("lead", [0, 1])
+@pytest.mark.parametrize("n", [1, 40, 2500])
+def test_token_counts_where_rows_share_words(ops, V, R, lead, n):
+    """rows that begin or end in the middle of a 32-bit word: ids counted exactly, also the first and the last of a row, up to 32767; what lies around stays"""
+    g = gen(V * 100 + R * 10 + lead)
+    buf = torch.full((lead + R * V + 3,), -21555, dtype=torch.int16, device="cuda")
+    counts = buf[lead:lead + R * V].view(R, V)
+    assert counts.data_ptr() % 4 == 2 * lead
+    counts.zero_()
+    counts[:, -1] = 32767 - 5
+    want = counts.long() & 0xffff
+    for prompt in (False, True, False):
+        ids = torch.randint(-1, V + 1, (R, n), generator=g, device="cuda").to(torch.int32)
+        ids[:, ::3] = torch.where(torch.rand((R, (n + 2) // 3), generator=g, device="cuda") < 0.5, 0, V - 1).to(torch.int32)
+        assert ops.token_counts_add(counts, ids, prompt=prompt) is counts
+        for r in range(R):
+            here = ids[r][(ids[r] >= 0) & (ids[r] < V)].long()
+            if prompt:
+                want[r, here] |= 0x8000
+            else:
+                want[r] = (want[r] & 0x8000) | ((want[r] & 0x7fff) + torch.bincount(here, minlength=V)).clamp_max(0x7fff)
+        assert torch.equal(counts.long() & 0xffff, want)
+    assert (buf[:lead] == -21555).all() and (buf[lead + R * V:] == -21555).all()
+    for token in (0, V - 1):                                     # the greedy choice counts there too
+        logits = torch.zeros((R, V), device="cuda")
+        logits[:, token] = 1
+        assert (ops.select_token(logits, counts=counts, update_counts=True) == token).all()
+        want[:, token] = (want[:, token] & 0x8000) | ((want[:, token] & 0x7fff) + 1).clamp_max(0x7fff)
+    assert torch.equal(counts.long() & 0xffff, want)
+    assert (buf[:lead] == -21555).all() and (buf[lead + R * V:] == -21555).all()
+
+
+def test_token_counts_of_neighbours_at_once(ops):
+    """two callers whose counts meet inside a 32-bit word, at the same time"""
+    V, n = 501, 4000
+    buf = torch.zeros((2 * V + 1,), dtype=torch.int16, device="cuda")
+    ids = torch.randint(0, V, (1, n), generator=gen(77), device="cuda").to(torch.int32)
+    ids[:, ::2], ids[:, 1::4] = 0, V - 1
+    parts = [buf[:V].view(1, V), buf[V:2 * V].view(1, V)]
+    torch.cuda.synchronize()
+    for p in parts:
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(4):
+                ops.token_counts_add(p, ids)
+    torch.cuda.synchronize()
+    want = (4 * torch.bincount(ids[0].long(), minlength=V))
+    assert all(torch.equal(p[0].long(), want) for p in parts) and int(buf[-1]) == 0
