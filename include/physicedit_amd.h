@@ -343,7 +343,8 @@ typedef struct pe_kv_append_args {
 int pe_kv_append_e4m3(const pe_kv_cache* cache, const pe_kv_append_args* a, void* stream);
 /* Attention of the T (1 ... 64) newest tokens, already appended at rows start[b] + t: query (b, t, h) sees the cache rows [0, start[b]) and the row
  * start[b] + j of every new token j with bit j of tree[b][t] set (device uint64 [batch][T]: the token's ancestors and, usually, itself); tree NULL =
- * causal.  Grouped heads: query head h reads kv head h / (n_q / n_kv).  softmax in fp32; a query that sees nothing, or start[b] < 0: zeros.
+ * causal.  Grouped heads: query head h reads kv head h / (n_q / n_kv).  softmax in fp32, divided once at the end: the visible |values| of a channel may sum
+ * up to 3.4e38 (beyond, the result can be infinite or NaN).  A query that sees nothing, or start[b] < 0: zeros.
  * q bf16 with strides {batch, token, head} (multiples of 8), out [batch][T][n_q][head_dim] bf16.  workspace: pe_kv_attention_workspace_bytes, 16-byte
  * aligned, private to the stream (a captured graph keeps its own). */
 size_t pe_kv_attention_workspace_bytes(int batch, int n_kv, int T, int n_q, int head_dim, int capacity);

@@ -223,7 +223,7 @@ int launch_kv_append(const KvAppend& in, hipStream_t stream) {
 // e4m3 -> bf16 is exact (v_cvt_scalef32_pk_bf16_fp8, two codes an instruction); scale_k multiplies the fp32 score, scale_v the fp32
 // probability.  The product p * scale_v goes into the matrix unit as TWO bf16, its rounding and the remainder: the matrix unit has time to spare here
 // and the sum then carries 16 bits of each term instead of 8.
-// Scores, maximum, sums and O are fp32.  A wave walks every fourth block of its work-group's range with a running maximum of its own; waves and
+// Scores, maximum, sums and O are fp32.  A wave walks every fourth block of its work-group's range with a reference of its own for the exponentials; waves and
 // work-groups (the cache's axis is split over `splits` of them) are joined in a fixed order.
 // ------------------------------------------------------------------------------------------------
 PE_DEV bf16x8 codes8(uint32_t a, uint32_t b) {
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(WR * WK * 64, 2) kv_attention_kernel(KvAttenti
     for (int s = 0; s < KS; ++s) qf[s] = *(const bf16x8*)(q + 64 * (s >> 1) + 8 * (s & 1));
     const unsigned long long word = a.tree ? a.tree[(size_t)b * a.T + t_q] : (2ull << t_q) - 1;
     f32x4 o[DT] = {};
-    float m = -INFINITY, l = 0.f;                                            // running maximum of the scores (times log2 e) and sum
+    float m = -INFINITY, l = 0.f;                                            // reference of the exponentials (scores times log2 e) and their sum
 
     auto work = [&](Block& t, int blk) __attribute__((always_inline)) {
         f32x4 s4[4] = {};                         // four independent accumulators in turn: an MFMA's result is not there for the next one
@@ -373,9 +373,10 @@ __global__ void __launch_bounds__(WR * WK * 64, 2) kv_attention_kernel(KvAttenti
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, s4[h][i]);
         top = max_over_j(top);
-        // the reference of the exponentials follows the maximum only when it falls 2^8 behind: probabilities up to 256 cost nothing in fp32, the rescaling does
-        if (__any(top > m + 8.f)) {
-            const float m_new = fmaxf(m, top);
+        // The reference of the exponentials is raised to 8 above the maximum where that has passed it, so most blocks find it high enough: the rescaling costs.
+        // Probabilities stay at or below 1 (the largest between 2^-8 and 1 when its block is done), so |O| never passes the sum of the visible |v|.
+        if (__any(top > m)) {
+            const float m_new = fmaxf(m, top + 8.f);
             const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m_new);        // 0 from -inf
             l *= alpha;
 #pragma unroll

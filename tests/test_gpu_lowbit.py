@@ -840,3 +840,36 @@ def test_token_counts_of_neighbours_at_once(ops):
     torch.cuda.synchronize()
     want = (4 * torch.bincount(ids[0].long(), minlength=V))
     assert all(torch.equal(p[0].long(), want) for p in parts) and int(buf[-1]) == 0
+
+
+@pytest.mark.parametrize("B,H,T,cap", [(64, 32, 1, 512), (128, 16, 3, 512), (1, 1, 5, 128), (1, 2, 40, 192)], ids=["1row", "2rowtiles", "4rowtiles", "40tokens"])
+@pytest.mark.parametrize("size", [1e37, 4e35, 1e-30])
+def test_kv_attention_values_of_any_size(ops, B, H, T, cap, size):
+    """scores that rise from block to block while the values are close to fp32's largest (as a sum: the documented limit) or far below one: the result is
+    their mean.  Each wave walks at least two blocks here."""
+    g = gen(T + cap)
+    G, D = 7, 64
+    cache = ops.KVCacheE4M3(B, H, cap, D)
+    n = cap - T
+    k, v = torch.zeros((2, B, cap, H, D), device="cuda")
+    k[..., 0] = torch.arange(cap, device="cuda").view(1, cap, 1) // 64 * (5.4 / (cap // 64 - 1))            # 7.8 in powers of two, from first block to last
+    v += (torch.rand((B, cap, H, D), generator=g, device="cuda") - 0.3) * (size if size < 1e36 else 1.0)
+    if size > 1e36:                                                                                          # one value of that size
+        v[:, n - 20, :, 3] = size
+    ops.kv_append_e4m3(cache, k.to(BF), v.to(BF), torch.zeros((B,), dtype=torch.int32, device="cuda"))
+    q = torch.zeros((B, T, H * G, D), device="cuda")
+    q[..., 0] = 1 + 0.01 * torch.arange(H * G, device="cuda") / (H * G)
+    q = q.to(BF)
+    start = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    got = ops.kv_attention_e4m3(q, cache, start, scale=1.0)
+    l = logical(cache)
+    for b, h in ((0, 0), (B - 1, H - 1)):
+        here = {x: t[b:b + 1, h:h + 1] for x, t in l.items()}
+        kk, vv = here["k"].to(F64) * here["k_scale"].to(F64)[..., None], here["v"].to(F64) * here["v_scale"].to(F64)[..., None]
+        for t in range(T):
+            s = q[b, t, h * G:(h + 1) * G].to(F64) @ kk[0, 0, :n + t + 1].T
+            p = torch.softmax(s, -1)
+            want, most = p @ vv[0, 0, :n + t + 1], p @ vv[0, 0, :n + t + 1].abs()
+            # as attention_reference: D products and four roundings of scores up to 5.5, p as two bf16, sums of n terms
+            near(got[b, t].view(H, G, D)[h], want, most * (2 * (D + 4) * 2.0 ** -24 * 5.5 + 2.0 ** -15 + n * 2.0 ** -24))
+    assert got.isfinite().all()
