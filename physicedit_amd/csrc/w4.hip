@@ -98,10 +98,15 @@ __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
     for (int kc = w; kc < a.KC; kc += W) {
         u32x4 wq[R], sc[R][GC];
         bf16x8 b[MT][4];
-        if (!AHEAD) PE_W4_FETCH(kc, wq, sc)
-        // x is in LDS when at most the R (1 + GC) younger loads are under way.  (The compiler's own wait for copies into LDS is not there in every variant.)
-        constexpr int YOUNGER = R * (1 + GC);
-        __builtin_amdgcn_s_waitcnt((YOUNGER & 15) | (YOUNGER >> 4) << 14 | 0x0f70);      // vmcnt(YOUNGER) alone
+        // The compiler's own waits between copies into LDS and reads of it are not there in every variant.  Each wait here is for everything, whatever loads
+        // the compiler emits beside them, and no memory access passes it: the last chunk's reads are done before its place is filled again, and the
+        // copies before they are read.  (A wait for the copies alone, by the number of younger loads, is no faster: 14.1, 13.1, 20.3 and 56.4 us against
+        // 14.3, 13.2, 20.4 and 55.9 -- N, K = 3584, 18944 with 7 rows, 5001, 3424 with 33, 3584, 18944 with 24, 152064, 3584 with one; gated, one row: 18.4, 18.5.)
+        if (!AHEAD) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            PE_W4_FETCH(kc, wq, sc)
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int s = 0; s < 4; ++s)
@@ -115,7 +120,7 @@ __global__ void __launch_bounds__(W * 64) gemv_w4_kernel(W4Args a) {
                 for (int g = 0; g < GC; ++g) sc[r][g] = ns[r][g];
             }
             __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_waitcnt(0x0070);         // vmcnt(0) lgkmcnt(0): the chunk is in registers, its place in LDS is free
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // the chunk is in registers, its place in LDS is free
             __builtin_amdgcn_sched_barrier(0);
             if (kc + W < a.KC) PE_W4_FETCH(kc + W, nq, ns)
         }
