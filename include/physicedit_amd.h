@@ -309,7 +309,8 @@ typedef struct pe_w4_weight {
     const void *codes, *scale;
     int N, K, group;
 } pe_w4_weight;
-/* out[M, N] = r * (x @ W^T) + bias + res for 1 ... 64 rows x [M,K] bf16 (finite values; row stride ldx, a multiple of 8; 16-byte aligned).  norm_eps >= 0:
+/* out[M, N] = r * (x @ W^T) + bias + res for 1 ... 64 rows x [M,K] bf16 (row stride ldx, a multiple of 8; 16-byte aligned; values up to 2^100 in size, up to
+ * 2^50 with norm_eps: a row that holds a larger one, an infinity or a NaN gives results that are not the definition's, and no other row does).  norm_eps >= 0:
  * r[m] = rsqrt(mean(x[m]^2) + norm_eps), an RMSNorm whose weight the caller folded into W; norm_eps < 0: r = 1.  bias [N], res [M, N] (row
  * stride ldr; may be out itself) nullable; out may not be x.  swiglu != 0: W holds the F = N / 2 gate rows, then the F up rows (F % 16 == 0), and
  * out[M, F] = silu(gate) * up (no res). */

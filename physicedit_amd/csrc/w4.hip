@@ -11,8 +11,10 @@
 // two instructions (a shift and an and-or).  The offset and the zero point leave through the row sum of x over the group,
 //   sum (c - z) x = sum (128 + c) x - (128 + z) sum x,
 // which one more MFMA per 32 inputs (ones as the weights) gives every lane for the rows it holds; products of two bf16 are exact in
-// fp32, so this costs about 2^-24 * 136 * sum |x| of a group, far below the output's bf16 rounding.  r comes the same way: x as BOTH
-// operands leaves sum x^2 on the diagonal.
+// fp32, so this costs about 2^-24 * 136 * sum |x| of a group, far below the output's bf16 rounding: of 25088 outputs at K = 18944, 42 round otherwise than
+// the exact value, 28 of the plain fp32 form's.  (In the mantissa of 16.0 it costs 24 instead of 136, 15 of 25088 round otherwise, and two more instructions a
+// code word and scale: gated, one row 18.3 -> 20.0 us; vocabulary 56.3 -> 58.9.)  r comes the same way: x as BOTH operands leaves sum x^2 on the diagonal.
+// 143 |x| summed over a group has to stay finite, and sum x^2 where it is asked for: |x| <= 2^100, or 2^50 with the norm, keeps all of them far from the end.
 //
 // Layout of the codes: tiles of 16 outputs x 128 inputs, 1 KiB, [N/16][K/128][lane][step]: the lane's four words are its A fragments of the
 // four 32-input steps (output lane & 15, inputs 32 step + 8 (lane >> 4) + e, element e in nibble (e >> 1) + 4 (e & 1)), one coalesced 16-byte load

@@ -611,8 +611,9 @@ def quantize_w4(w: torch.Tensor, group: int = 128, zero_point: bool = True, norm
 
 def gemv_w4(x: torch.Tensor, w: W4Weight, bias: Optional[torch.Tensor] = None, res: Optional[torch.Tensor] = None, epilogue: str = "bias",
             norm_eps: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """x [M, K] or [K] (M <= 64 rows of finite values; a row stride is fine) @ w.T + bias + res -> [M, N] or [N], one rounding.  epilogue="swiglu": w holds the gate
-    rows, then as many up rows (a multiple of 16): silu(gate) * up.  norm_eps: x is RMS-normalised (its norm weight folded into w)."""
+    """x [M, K] or [K] (M <= 64 rows; a row stride is fine) @ w.T + bias + res -> [M, N] or [N], one rounding.  epilogue="swiglu": w holds the gate
+    rows, then as many up rows (a multiple of 16): silu(gate) * up.  norm_eps: x is RMS-normalised (its norm weight folded into w).  Values of x up to
+    2^100 in size, 2^50 with norm_eps; a row that holds larger ones is not the definition's (infinite or NaN), the others are."""
     if epilogue != "bias" and epilogue != "swiglu":
         raise ValueError(f"gemv_w4: epilogue {epilogue!r} ('bias' or 'swiglu')")
     if norm_eps is not None and not norm_eps >= 0:

@@ -873,3 +873,71 @@ def test_kv_attention_values_of_any_size(ops, B, H, T, cap, size):
             # as attention_reference: D products and four roundings of scores up to 5.5, p as two bf16, sums of n terms
             near(got[b, t].view(H, G, D)[h], want, most * (2 * (D + 4) * 2.0 ** -24 * 5.5 + 2.0 ** -15 + n * 2.0 ** -24))
     assert got.isfinite().all()
+
+
+@pytest.mark.parametrize("M,N,K,group,swiglu", [(1, 300, 2048, 64, False), (1, 3584, 18944, 128, False), (5, 4099, 640, 128, False), (20, 1000, 1408, 64, True),
+                                                (33, 8200, 384, 32, False), (64, 96, 4096, 32, True)])
+@pytest.mark.parametrize("norm", [False, True])
+def test_gemv_w4_range_of_inputs(ops, M, N, K, group, swiglu, norm):
+    """inputs of the documented largest size, 2^100 (2^50 with the norm), and tiny ones; scales bring the products back to about one.  A row beyond the range
+    touches no other."""
+    if swiglu:
+        N = N // 32 * 32
+    g = gen(N + K)
+    codes, scale, z, x = w4_case(g, M, N, K, group, True)
+    size = 50 if norm else 100
+    for e in (size, -size):
+        xe = (x.clamp(-1, 1) * 2.0 ** e).to(BF)
+        xe[:, ::5] = 2.0 ** e
+        se = scale if norm else (scale.float() * 2.0 ** -e).to(BF)                # the normalised rows are of about one already
+        w, plain = ops.pack_w4(codes, se, z, group), w4_weight(codes, se, z, group)
+        kw = dict(epilogue="swiglu" if swiglu else "bias", norm_eps=2.0 ** -120 if norm else None)
+        got = ops.gemv_w4(xe, w, **kw)
+        near(got, *w4_reference(plain, se, group, xe, 2.0 ** -120 if norm else None, None, None, swiglu))
+        if M > 1:
+            for big in (3.3e38, math.inf, math.nan):
+                x2 = xe.clone()
+                x2[M // 2, K // 3] = big
+                again = ops.gemv_w4(x2, w, **kw)
+                ok = torch.arange(M, device="cuda") != M // 2
+                assert torch.equal(again[ok], got[ok])
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", [(1, 300, 2048), (5, 4099, 640), (7, 3584, 18944), (20, 1000, 1408), (33, 8200, 384), (64, 96, 18944)])
+def test_gemv_w4_to_the_last_bit(ops, group, M, N, K):
+    """Inputs of 20 ... 57 whose weights are zero beside sixteenths whose weights are one: every sum that the kernel forms, (128 + code) x and x over a group,
+    is a multiple of 2^-4 below 143 * 57 * 128 < 2^20, so nothing is rounded before the result: a term lost or taken twice anywhere shows."""
+    g = gen(N + group)
+    G = K // group
+    z = torch.randint(1, 15, (N, G), generator=g, device="cuda")
+    codes = z.repeat_interleave(group, 1)
+    x = torch.randint(20, 58, (M, K), generator=g, device="cuda").float()
+    at = torch.arange(G, device="cuda") * group + torch.randint(0, group, (G,), generator=g, device="cuda")      # one input of every group
+    on = torch.rand((N, G), generator=g, device="cuda") < max(4.0 / G, 0.1)                                     # some of them count
+    x[:, at] = torch.randint(-15, 16, (M, G), generator=g, device="cuda").float() / 16
+    codes[:, at] += torch.where(on, torch.where(torch.rand((N, G), generator=g, device="cuda") < 0.5, 1, -1), 0)
+    scale = 2.0 ** torch.randint(-3, 1, (N, 1), generator=g, device="cuda").float().expand(N, G)
+    w = ops.pack_w4((codes[:, 0::2] | (codes[:, 1::2] << 4)).to(torch.uint8), scale.to(BF).contiguous(), z.to(torch.uint8), group)
+    want = x.to(F64) @ ((codes - z.repeat_interleave(group, 1)).to(F64) * scale.to(F64).repeat_interleave(group, 1)).T
+    assert torch.equal(ops.gemv_w4(x.to(BF), w), want.float().to(BF))
+
+
+@pytest.mark.parametrize("M,N,K,group", [(1, 3584, 18944, 128), (7, 3584, 18944, 64), (24, 3584, 18944, 32), (64, 3584, 18944, 128), (33, 5001, 3424, 32), (1, 37888, 3584, 128)])
+def test_gemv_w4_every_output(ops, M, N, K, group):
+    """Each output within half a step of bf16 and what fp32 can lose on the way.  A group: group / 8 roundings of partial sums of at most 143 sum |x| (an
+    instruction rounds four times in 32 terms or less), the same for sum x times 143, and two more; the groups' errors are independent and of no
+    preferred sign, as are the roundings of their running sum, which stays within sqrt(G) times the largest term or so of the result: six times the root of the
+    sum of squares covers all outputs."""
+    g = gen(K + M)
+    codes, scale, z, x = w4_case(g, M, N, K, group, True)
+    got = ops.gemv_w4(x, ops.pack_w4(codes, scale, z, group)).to(F64)
+    w = w4_weight(codes, scale, z, group)
+    want = x.to(F64) @ w.T
+    G, s = K // group, scale.to(F64)
+    xa = x.to(F64).abs().view(M, G, group).sum(2)
+    of_groups = ((xa * (2 * (group / 8) + 2) * 143 * 2.0 ** -24).square() @ s.square().T).sqrt()
+    of_sums = (G + 16) ** 0.5 * 2.0 ** -24 * (want.abs() + (G * ((x.to(F64).square() @ w.square().T))).sqrt())
+    loss = 6 * (of_groups + of_sums)
+    assert ((got - want).abs() <= HALF_BF * (want.abs() + loss) + loss).all()
+    assert float(loss.max() / want.std()) < 0.02                     # far below what one wrong term does
