@@ -157,6 +157,12 @@ double number(PyObject* o) {
     return v;
 }
 
+bool truth(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw Raise{nullptr, ""};
+    return v == 1;
+}
+
 // gemv_w4(x, address of the pe_w4_weight, its device, bias, res, swiglu, norm_eps, out)
 PyObject* gemv_w4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!count_ok(n, 8, "gemv_w4")) return nullptr;
@@ -165,7 +171,7 @@ PyObject* gemv_w4(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const pe_w4_weight* w = record<pe_w4_weight>(a[1]);
         const long dev = integer(a[2]);
         void* stream = stream_of(dev, "w");
-        const bool swiglu = PyObject_IsTrue(a[5]) == 1;
+        const bool swiglu = truth(a[5]);
         const int64_t dims = x.dim(), K = w->K, cols = swiglu ? w->N / 2 : w->N;
         if (x.scalar_type() != at::kBFloat16 || (dims != 1 && dims != 2) || x.size(-1) != K || x.stride(-1) != 1 || !on(x, (int)dev))
             bad("gemv_w4: expected bf16 rows of %lld contiguous values on cuda:%ld, got %s", (long long)K, dev, show(x).c_str());
@@ -325,7 +331,7 @@ PyObject* select_token(PyObject*, PyObject* const* a, Py_ssize_t n) {
         void* stream;
         const pe_logits_args s = logits_args(a, dev, stream);
         const at::Tensor& x = tensor(a[0], "logits");
-        const bool update = PyObject_IsTrue(a[5]) == 1;
+        const bool update = truth(a[5]);
         if (update && !s.counts) bad("select_token: update_counts without counts");
         int* to = (int*)at_(a[6], "out", at::kInt, {s.rows}, dev);
         int *ids = nullptr, *step = nullptr;
@@ -376,7 +382,7 @@ PyObject* token_counts_add(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int64_t R = c.size(0), V = c.size(1), m = t.size(1);
         void* cp = at_(a[0], "counts", at::kShort, {R, V}, dev);
         const int* tp = (const int*)at_(a[1], "tokens", at::kInt, {R, m}, dev);
-        const bool prompt = PyObject_IsTrue(a[2]) == 1;
+        const bool prompt = truth(a[2]);
         launch("pe_token_counts_add", [&] { return api.token_counts_add(cp, V, (int)R, (int)V, tp, (int)m, prompt, stream); });
         Py_INCREF(a[0]);
         return a[0];

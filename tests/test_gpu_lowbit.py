@@ -941,3 +941,13 @@ def test_gemv_w4_every_output(ops, M, N, K, group):
     loss = 6 * (of_groups + of_sums)
     assert ((got - want).abs() <= HALF_BF * (want.abs() + loss) + loss).all()
     assert float(loss.max() / want.std()) < 0.02                     # far below what one wrong term does
+
+
+def test_flags_that_have_no_truth(ops):
+    """a flag that cannot be read as true or false is its own error, and nothing is launched"""
+    counts, both = torch.zeros((1, 40), dtype=torch.int16, device="cuda"), torch.ones(2)
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        ops.token_counts_add(counts, torch.tensor([[3, 4]], dtype=torch.int32, device="cuda"), prompt=both)
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        ops.select_token(torch.zeros((1, 40), device="cuda"), counts=counts, update_counts=both)
+    assert not counts.any()
