@@ -93,16 +93,16 @@ void* heads_(const at::Tensor& t, const char* name, at::IntArrayRef shape, long 
     return p;
 }
 
-// A result that the caller passed lies apart from input `in` -- or, where `over` says that each of its elements is read before it is written, exactly over it.
+// What a call writes for the caller (`result`: out, a workspace, counts) lies apart from input `in` -- or, where `over` says that each of its elements is read before it is written, exactly over it.
 // A dimension of strides counts with all that lies between its ends.
-void apart(PyObject* result, PyObject* in, const char* name, bool over = false) {
+void apart(PyObject* result, PyObject* in, const char* name, bool over = false, const char* what = "out") {
     if (result == Py_None || in == Py_None) return;
-    const at::Tensor &r = tensor(result, "out"), &t = tensor(in, name);
+    const at::Tensor &r = tensor(result, what), &t = tensor(in, name);
     int64_t span = 1;
     for (int64_t i = 0; i < t.dim(); ++i) span += (t.size(i) - 1) * t.stride(i);
     const char *r0 = (const char*)r.data_ptr(), *t0 = (const char*)t.data_ptr(), *r1 = r0 + r.nbytes(), *t1 = t0 + span * (int64_t)t.element_size();
     if (r1 <= t0 || t1 <= r0 || (over && r0 == t0 && t.is_contiguous() && t.nbytes() == r.nbytes())) return;
-    bad("out: overlaps %s%s", name, over ? " (it may only lie exactly over it)" : "");
+    bad("%s: overlaps %s%s", what, name, over ? " (it may only lie exactly over it)" : "");
 }
 
 const at::Tensor& four_dims(PyObject* o, const char* name, const char* what) {
@@ -232,6 +232,8 @@ PyObject* kv_append_e4m3(PyObject*, PyObject* const* a, Py_ssize_t n) {
             apart(a[9], a[3], "v");
             apart(a[9], a[6], "cos");
             apart(a[9], a[7], "sin");
+            apart(a[9], a[4], "start");
+            apart(a[9], a[8], "positions");
         }
         launch("pe_kv_append_e4m3", [&] { return api.kv_append_e4m3(c, &s, stream); });
         if (!has_q) Py_RETURN_NONE;
@@ -257,7 +259,12 @@ PyObject* kv_attention_e4m3(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const float scale = a[5] == Py_None ? (float)(1.0 / std::sqrt((double)D)) : (float)number(a[5]);
         void* to = at_(a[6], "out", at::kBFloat16, {B, T, nq * D}, dev);
         apart(a[6], a[0], "q", true);
-        apart(a[6], a[7], "workspace");
+        apart(a[6], a[3], "start");
+        apart(a[6], a[4], "tree");
+        apart(a[7], a[6], "out", false, "workspace");
+        apart(a[7], a[0], "q", false, "workspace");
+        apart(a[7], a[3], "start", false, "workspace");
+        apart(a[7], a[4], "tree", false, "workspace");
         at::Tensor out, ws;
         if (a[6] == Py_None) { out = empty_like_type(q, {B, T, nq * D}, at::kBFloat16); to = out.data_ptr(); }
         void* wp = nullptr;
@@ -348,7 +355,9 @@ PyObject* select_token(PyObject*, PyObject* const* a, Py_ssize_t n) {
             apart(a[6], a[i], names[i]);
             apart(a[7], a[i], names[i]);
             apart(a[8], a[i], names[i]);
+            apart(a[9], a[i], names[i], false, "workspace");
         }
+        for (int i = 6; i < 9; ++i) apart(a[9], a[i], i == 6 ? "out" : i == 7 ? "out_ids" : "step", false, "workspace");
         apart(a[6], a[7], "out_ids");
         apart(a[6], a[8], "step");
         apart(a[7], a[8], "step");
@@ -382,6 +391,7 @@ PyObject* token_counts_add(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int64_t R = c.size(0), V = c.size(1), m = t.size(1);
         void* cp = at_(a[0], "counts", at::kShort, {R, V}, dev);
         const int* tp = (const int*)at_(a[1], "tokens", at::kInt, {R, m}, dev);
+        apart(a[0], a[1], "tokens", false, "counts");
         const bool prompt = truth(a[2]);
         launch("pe_token_counts_add", [&] { return api.token_counts_add(cp, V, (int)R, (int)V, tp, (int)m, prompt, stream); });
         Py_INCREF(a[0]);

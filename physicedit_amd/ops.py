@@ -501,7 +501,7 @@ def sdpa_heads64(q: torch.Tensor, kv: torch.Tensor, heads: int) -> torch.Tensor:
 
 # ---- the low-bit decode step: 4-bit linears, the e4m3 key/value cache, next-token scores (include/physicedit_amd.h) -----------------
 # Their checks, allocations and launches are in csrc/binding.cpp (_lib.binding()); laying a weight out is here.
-# A result passed as `out` lies apart from the inputs, or exactly over gemv_w4's res, kv_append_e4m3's or kv_attention_e4m3's q, process_logits' logits or bias.
+# A result passed as `out`, and a workspace, lie apart from the inputs and from one another; `out` may lie exactly over gemv_w4's res, kv_append_e4m3's or kv_attention_e4m3's q, process_logits' logits or bias.
 def _stream_of(dev: int, name: str) -> int:
     """the current stream of device `dev`, which has to be the current device"""
     if dev < 0:

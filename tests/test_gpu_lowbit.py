@@ -951,3 +951,42 @@ def test_flags_that_have_no_truth(ops):
     with pytest.raises(RuntimeError, match="ambiguous"):
         ops.select_token(torch.zeros((1, 40), device="cuda"), counts=counts, update_counts=both)
     assert not counts.any()
+
+
+def test_what_a_call_writes_lies_apart_from_all_it_reads(ops):
+    """the small inputs too (row counters, trees, positions, ids), and the workspace: every overlap is refused before a launch"""
+    raw = torch.zeros((1 << 16,), dtype=torch.uint8, device="cuda")
+    view = lambda lo, dtype, *shape: raw[lo:lo + math.prod(shape) * dtype.itemsize].view(dtype).view(shape)
+    B, T, hq, hkv, D = 2, 3, 4, 2, 64
+    cache = ops.KVCacheE4M3(B, hkv, 1024, D)
+    cos, sin = tables(1024, D, BF)
+    k, q, start = torch.zeros((B, T, hkv, D), dtype=BF, device="cuda"), torch.zeros((B, T, hq, D), dtype=BF, device="cuda"), torch.zeros((B,), dtype=torch.int32, device="cuda")
+    out4, out3 = view(0, BF, B, T, hq, D), view(0, BF, B, T, hq * D)
+    inside = 64
+    positions, tree = view(inside, torch.int32, B, T), view(inside, torch.int64, B, T)
+    ws = raw[:ops.kv_attention_workspace(cache, T, hq).numel()]
+    assert ws.numel() > 0
+    V, wide = 20000, torch.zeros((1, 20000), device="cuda")
+    counts = torch.zeros((1, V), dtype=torch.int16, device="cuda")
+    sel = raw[:16384]
+    one = lambda at: view(at, torch.int32, 1)
+    calls = {
+        "out: overlaps start": [lambda: ops.kv_append_e4m3(cache, k, k, view(inside, torch.int32, B), q=q, cos=cos, sin=sin, out=out4),
+                                lambda: ops.kv_attention_e4m3(q, cache, view(inside, torch.int32, B), out=out3)],
+        "out: overlaps positions": [lambda: ops.kv_append_e4m3(cache, k, k, start, q=q, cos=cos, sin=sin, positions=positions, out=out4)],
+        "out: overlaps tree": [lambda: ops.kv_attention_e4m3(q, cache, start, tree=tree, out=out3)],
+        "workspace: overlaps out": [lambda: ops.kv_attention_e4m3(q, cache, start, out=out3, workspace=ws), lambda: ops.select_token(wide, out=one(8), workspace=sel)],
+        "workspace: overlaps q": [lambda: ops.kv_attention_e4m3(view(0, BF, B, T, hq, D), cache, start, workspace=ws)],
+        "workspace: overlaps start": [lambda: ops.kv_attention_e4m3(q, cache, view(inside, torch.int32, B), workspace=ws)],
+        "workspace: overlaps tree": [lambda: ops.kv_attention_e4m3(q, cache, start, tree=tree, workspace=ws)],
+        "workspace: overlaps logits": [lambda: ops.select_token(view(0, torch.float32, 1, 10000), workspace=sel)],
+        "workspace: overlaps counts": [lambda: ops.select_token(view(32768, torch.float32, 1, 8192)[:, :8192], counts=view(0, torch.int16, 1, 8192), workspace=sel)],
+        "workspace: overlaps allowed": [lambda: ops.select_token(wide, allowed=view(0, torch.int32, (V + 31) // 32), workspace=sel)],
+        "workspace: overlaps step": [lambda: ops.select_token(wide, out_ids=torch.zeros(4, dtype=torch.int32, device="cuda"), step=one(8), workspace=sel)],
+        "workspace: overlaps out_ids": [lambda: ops.select_token(wide, out_ids=one(12), step=torch.zeros(1, dtype=torch.int32, device="cuda"), workspace=sel)],
+        "counts: overlaps tokens": [lambda: ops.token_counts_add(view(0, torch.int16, 1, 100), view(8, torch.int32, 1, 4))]}
+    for text, fs in calls.items():
+        for f in fs:
+            with pytest.raises(ValueError, match=text):
+                f()
+    assert not raw.any() and not counts.any()
