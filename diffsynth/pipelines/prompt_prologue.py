@@ -676,13 +676,12 @@ class GraphDecoder:
                         raise RuntimeError("pe_decode_layer: a grid barrier timed out (the decode grid was not fully resident); "
                                            "set PE_DECODE_LAYER_KERNEL=0")
                     done += n
-                    if select and min(new) < 0:
-                        raise RuntimeError("GraphDecoder.generate: no token is allowed")
                     stop = next((i for i, t in enumerate(new) if t in eos), None)
+                    tokens += new if stop is None else new[:stop + 1]               # what came behind EOS was never asked for
+                    if select and min(tokens) < 0:
+                        raise RuntimeError("GraphDecoder.generate: no token is allowed")
                     if stop is not None:
-                        tokens += new[:stop + 1]
                         break
-                    tokens += new
             torch.cuda.current_stream(dev).wait_stream(side)
         return torch.cat([ids, torch.tensor([tokens], dtype=ids.dtype, device=ids.device)], dim=1)
 

@@ -335,3 +335,24 @@ def test_old_copies_go_before_new_ones_come(model, config, weights, kv_cache):
         assert other <= first + held // 8
     finally:
         dec.reset()
+
+
+def test_nothing_behind_eos_counts(model, config):
+    """the steps that a chunk runs past EOS may find no token at all (scores of NaN here): the answer ended before them"""
+    dec = decoder(model)
+    inputs = prompt(37)
+    config.repetition_penalty = 1.3
+    free = dec.generate(max_new_tokens=12, **inputs)
+    config.eos_token_id = int(free[0, 37 + 3])
+    table = model.model.language_model.embed_tokens.weight
+    kept = table[config.eos_token_id].clone()
+    try:
+        with torch.no_grad():
+            table[config.eos_token_id] = float("nan")
+        assert torch.equal(dec.generate(max_new_tokens=12, **inputs), free[:, :37 + 4])
+        config.eos_token_id = None
+        with pytest.raises(RuntimeError, match="no token is allowed"):
+            dec.generate(max_new_tokens=12, **inputs)
+    finally:
+        with torch.no_grad():
+            table[int(free[0, 37 + 3])] = kept
