@@ -356,3 +356,56 @@ def test_nothing_behind_eos_counts(model, config):
     finally:
         with torch.no_grad():
             table[int(free[0, 37 + 3])] = kept
+
+
+@torch.no_grad()
+def test_four_bit_copies_stand_for_the_model(model):
+    """each 4-bit copy of the step against the model's own tensors: the right matrices in the right order with the right norm's weight in the columns.
+    Elementwise: half a step, a scale rounded to bf16 (15 steps / 256) and a zero point rounded to a whole number (half a step), as quantize_w4's own test
+    has it.  By column, over N outputs: the copy regressed on the model's weight gives the norm's weight, 1 +- 0.1, up to the quantisation's noise, below
+    0.4 of a weight's deviation in each output (a step of (max - min) / 15 of 128 normal values, 0.4, over sqrt 12, the roundings above added), divided by
+    sqrt N; six times that."""
+    dec = decoder(model, weights="w4", kv_cache="e4m3")
+    dec.generate(max_new_tokens=2, **prompt(20, 1))
+    _, layers, head = dec._w4
+    norms = [ly.input_layernorm.weight for ly in dec.layers] + [ly.post_attention_layernorm.weight for ly in dec.layers] + [dec.lm.norm.weight]
+    assert all((a.float() - b.float()).std() > 0.1 for i, a in enumerate(norms) for b in norms[:i])          # told apart below
+
+    def check(copy, weight, norm):
+        got, w = dequantised(copy), weight.to(F64)
+        n = torch.ones(w.shape[1], dtype=F64, device="cuda") if norm is None else norm.to(F64)
+        assert got.shape == w.shape
+        exact = w * n
+        parts = exact.view(exact.shape[0], -1, copy.group)
+        step = ((parts.amax(-1).clamp_min(0) - parts.amin(-1).clamp_max(0)) / 15).repeat_interleave(copy.group, 1)
+        assert ((got - exact).abs() <= step * (1.0 + 15 / 256) + 1e-12).all()
+        column = (got * w).sum(0) / w.square().sum(0)
+        assert ((column - n).abs() <= 6 * 0.4 / w.shape[0] ** 0.5).all()
+    for (qkv, bias, o, gate_up, down), ly in zip(layers, dec.layers):
+        at, mlp = ly.self_attn, ly.mlp
+        check(qkv, torch.cat([at.q_proj.weight, at.k_proj.weight, at.v_proj.weight]), ly.input_layernorm.weight)
+        assert torch.equal(bias, torch.cat([at.q_proj.bias, at.k_proj.bias, at.v_proj.bias]))
+        check(o, at.o_proj.weight, None)
+        check(gate_up, torch.cat([mlp.gate_proj.weight, mlp.up_proj.weight]), ly.post_attention_layernorm.weight)
+        check(down, mlp.down_proj.weight, None)
+    check(head, model.lm_head.weight, dec.lm.norm.weight)
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("weights", ["bf16", "w4"])
+def test_the_prefill_reaches_the_cache(model, weights):
+    """the cache's rows after the prefill against the keys and values of the model's own pass: e4m3's half step of each value (2^-4 of it, 2^-10 of the row's
+    scale below the smallest normal code) and one of bf16 for a pass whose sums ran in another order"""
+    n = 150
+    inputs = prompt(n, 8)
+    dec = decoder(model, weights=weights, kv_cache="e4m3")
+    dec.generate(max_new_tokens=1, **inputs)
+    past = model(**inputs, use_cache=True, logits_to_keep=1).past_key_values
+    caches = next(iter(dec._static.values()))["cache"]
+    assert len(caches) == 3
+    for layer, c in zip(past.layers, caches):
+        for want, codes, scale in ((layer.keys, c.k, c.k_scale), (layer.values, c.v.reshape(1, 4, -1, 128), c.v_scale)):
+            s = scale[0, :, :n, None].to(F64)
+            got, want = codes[0, :, :n].to(F64) * s, want[0].to(F64)
+            assert ((got - want).abs() <= (2.0 ** -4 + 2.0 ** -7) * want.abs() + (2.0 ** -10 + 448 * 2.0 ** -7 / 64) * s).all()
+            assert (got - want).norm() <= 2.0 ** -4 * want.norm() and not codes[0, :, n:].to(F64).any()
