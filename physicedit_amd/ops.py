@@ -562,6 +562,8 @@ def pack_w4(codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tenso
         raise ValueError(f"pack_w4: K={K} must be a multiple of the group {group}")
     _at(codes, "codes", torch.uint8, (N, K // 2), dev.index), _at(scale, "scale", BF, (N, K // group), dev.index)
     _at(zero, "zero", torch.uint8, (N, K // group), dev.index)
+    if zero is not None and bool((zero > 15).any()):
+        raise ValueError("pack_w4: zero points above 15")
     tiles, chunks = (N + 15) // 16, (K + 127) // 128
     full = torch.zeros((tiles * 16, chunks * 64), dtype=torch.uint8, device=dev)
     full[:N, :K // 2] = codes
@@ -574,7 +576,7 @@ def pack_w4(codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tenso
 
     pair = torch.zeros((tiles * 16, chunks * (128 // group), 2), dtype=BF, device=dev)      # scale, -(128 + zero)
     pair[:N, :K // group, 0] = scale
-    pair[:N, :K // group, 1] = -136.0 if zero is None else -128.0 - (zero & 15).to(BF)
+    pair[:N, :K // group, 1] = -136.0 if zero is None else -128.0 - zero.to(BF)
     pair = pair.view(tiles, 16, -1, 2).transpose(1, 2).contiguous()
     return W4Weight(words.view(tiles, chunks, 64, 16), pair, N, K, group)
 

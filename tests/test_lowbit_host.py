@@ -192,3 +192,16 @@ def test_weights_and_caches_hold_their_buffers():
 def test_gemv_w4_eps_is_a_number(lib):
     """a NaN is not "no norm" """
     refused(lib, lib.pe_gemv_w4(P, 256, 1, C.byref(w4()), None, None, 32, 2 * P, 32, 0, float("nan"), None), "norm_eps")
+
+
+def test_pack_w4_zero_points_are_codes(monkeypatch):
+    """a zero point above 15 is refused, not cut to four bits"""
+    from physicedit_amd import ops
+    monkeypatch.setattr(ops, "_stream_of", lambda dev, name: 0)
+    monkeypatch.setattr(ops, "_at", lambda t, *a: None)
+    codes, scale = torch.zeros((16, 64), dtype=torch.uint8), torch.ones((16, 1), dtype=BF)
+    zero = torch.full((16, 1), 15, dtype=torch.uint8)
+    assert float(ops.pack_w4(codes, scale, zero).scale[0, 0, 3, 1]) == -143
+    zero[7] = 16
+    with pytest.raises(ValueError, match="above 15"):
+        ops.pack_w4(codes, scale, zero)
