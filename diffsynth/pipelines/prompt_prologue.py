@@ -363,6 +363,10 @@ class GraphDecoder:
     MAX_CACHE_ROWS_E4M3 = 1 << 30   # KVCacheE4M3's: memory ends first
 
     @property
+    def low_bit(self) -> bool:
+        return (self.weights, self.kv_cache) != ("bf16", "bf16")
+
+    @property
     def max_rows(self) -> int:
         """prompt + new tokens that the captured step has room for"""
         return self.MAX_CACHE_ROWS if self.kv_cache == "bf16" else self.MAX_CACHE_ROWS_E4M3
@@ -767,7 +771,8 @@ class PromptPrologue:
                  decode_graph: bool = True, decode_weights: Optional[str] = None, decode_kv_cache: Optional[str] = None):
         """decode_weights / decode_kv_cache: GraphDecoder's weights ("bf16", "w4") and kv_cache ("bf16", "e4m3"); by default the environment's
         PE_DECODE_WEIGHTS / PE_DECODE_KV_CACHE, else bf16.  What is chosen there is used or refused (ValueError): only bf16 falls back to
-        transformers' generate() where the captured step is not available or switched off."""
+        transformers' generate() where the captured step is not available or switched off.  A call whose generation config asks for more than
+        that step applies runs transformers' bf16 generate() and says so."""
         low_bit = GraphDecoder.choice(decode_weights, decode_kv_cache) != ("bf16", "bf16")
         self.text_encoder = text_encoder
         self.decode_gemv = 0
@@ -836,6 +841,8 @@ class PromptPrologue:
         if (self.graph_decoder is not None and _captured_step_covers(gen) and ids.shape[0] == 1
                 and ids.shape[1] + max_new_tokens <= self.graph_decoder.max_rows):        # longer: the reference's own path
             return self.graph_decoder.generate(max_new_tokens=max_new_tokens, prefix_allowed_tokens_fn=prefix_allowed_tokens_fn, **model_inputs)
+        if self.graph_decoder is not None and self.graph_decoder.low_bit:
+            print("[prompt_prologue] this call's generation config, batch or length is not the captured decode step's: bf16 weights and cache, generate()")
         more = {} if prefix_allowed_tokens_fn is None else {"prefix_allowed_tokens_fn": prefix_allowed_tokens_fn}
         if getattr(gen, "stop_strings", None):
             more["tokenizer"] = self.tokenizer

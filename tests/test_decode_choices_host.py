@@ -10,7 +10,7 @@ from diffsynth.pipelines import prompt_prologue as PP
 
 class Recorder:
     """stands for the captured decoder and for the text encoder: notes which of them was asked, and how"""
-    max_rows = PP.GraphDecoder.MAX_CACHE_ROWS
+    max_rows, low_bit = PP.GraphDecoder.MAX_CACHE_ROWS, False
 
     def __init__(self, calls, name):
         self.calls, self.name = calls, name
@@ -126,3 +126,13 @@ def test_the_caches_have_limits_of_their_own():
         pp.generate_ids(long, 1000)
         pp.generate_ids(long, 360)
         assert [c[0] for c in calls] == [path, "captured"]
+
+
+def test_a_low_bit_decoder_that_is_passed_over_says_so(capsys):
+    for weights, kv_cache, told in (("bf16", "bf16", False), ("bf16", "e4m3", True), ("w4", "e4m3", True)):
+        for config, inputs, path in ((dict(no_repeat_ngram_size=2), INPUTS, "transformers"), (dict(), dict(input_ids=torch.zeros((2, 5), dtype=torch.long)), "transformers"),
+                                     (dict(), INPUTS, "captured")):
+            pp, calls = prologue(**config)
+            pp.graph_decoder.low_bit = PP.GraphDecoder.low_bit.fget(types.SimpleNamespace(weights=weights, kv_cache=kv_cache))
+            pp.generate_ids(inputs, 9)
+            assert calls[0][0] == path and ("bf16 weights" in capsys.readouterr().out) == (told and path == "transformers")
