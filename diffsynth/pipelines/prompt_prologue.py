@@ -410,7 +410,7 @@ class GraphDecoder:
         if self.layer_kernel and self.kv_cache != "bf16":
             raise ValueError("GraphDecoder: PE_DECODE_LAYER_KERNEL=1 is the bf16 step's")
         hidden, ff = self.lm.embed_tokens.weight.shape[1], self.layers[0].mlp.gate_proj.out_features
-        if self.weights == "w4" and (hidden % w4_group or ff % w4_group or ff % 16 or (at.q_proj.out_features % w4_group)):
+        if self.weights == "w4" and (w4_group not in (32, 64, 128) or hidden % w4_group or ff % w4_group or ff % 16 or (at.q_proj.out_features % w4_group)):
             raise ValueError(f"GraphDecoder: hidden {hidden}, MLP {ff} and groups of {w4_group} do not fit weights='w4'")
         self._layer_w = None        # per layer: the C struct of its operands (addresses: rebuilt when the weights' fingerprint changes)
         self.split_attention = os.environ.get("PE_DECODE_SPLIT_ATTENTION", "1") != "0"  # pe_decode_step_attention_split (448 work-groups per launch) instead of the 28-work-group launch; same bits

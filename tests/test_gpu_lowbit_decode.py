@@ -409,3 +409,10 @@ def test_the_prefill_reaches_the_cache(model, weights):
             got, want = codes[0, :, :n].to(F64) * s, want[0].to(F64)
             assert ((got - want).abs() <= (2.0 ** -4 + 2.0 ** -7) * want.abs() + (2.0 ** -10 + 448 * 2.0 ** -7 / 64) * s).all()
             assert (got - want).norm() <= 2.0 ** -4 * want.norm() and not codes[0, :, n:].to(F64).any()
+
+
+def test_a_group_that_no_kernel_takes_is_refused_at_once(model):
+    for group in (16, 256, 512, 0):
+        with pytest.raises(ValueError, match="groups of"):
+            decoder(model, weights="w4", kv_cache="e4m3", w4_group=group)
+    assert decoder(model, weights="w4", kv_cache="e4m3", w4_group=32).w4_group == 32
