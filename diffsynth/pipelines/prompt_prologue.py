@@ -681,8 +681,9 @@ class GraphDecoder:
                                            "set PE_DECODE_LAYER_KERNEL=0")
                     done += n
                     stop = next((i for i, t in enumerate(new) if t in eos), None)
-                    tokens += new if stop is None else new[:stop + 1]               # what came behind EOS was never asked for
-                    if select and min(tokens) < 0:
+                    new = new if stop is None else new[:stop + 1]                   # what came behind EOS was never asked for
+                    tokens += new
+                    if select and min(new) < 0:
                         raise RuntimeError("GraphDecoder.generate: no token is allowed")
                     if stop is not None:
                         break
